@@ -66,6 +66,50 @@ class GpoArgs(ctypes.Structure):
     ]
 
 
+class GpoHeads(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("stride_batch", ctypes.c_int64),
+                ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
+class GpoWindowArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32), ("batch", ctypes.c_int64), ("q_len", ctypes.c_int64),
+        ("kv_len", ctypes.c_int64), ("window", ctypes.c_int64), ("sinks", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("q", GpoHeads), ("k", GpoHeads), ("v", GpoHeads), ("out", GpoHeads),
+        ("lse", ctypes.c_void_p), ("dout", GpoHeads), ("dq", GpoHeads), ("dk", GpoHeads),
+        ("dv", GpoHeads), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class GpoPagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32), ("num_seqs", ctypes.c_int64), ("tokens", ctypes.c_int64),
+        ("max_q", ctypes.c_int64), ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+        ("table_width", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+        ("window", ctypes.c_int64), ("sinks", ctypes.c_int64), ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32), ("q", GpoHeads), ("out", GpoHeads), ("k_pages", GpoHeads),
+        ("v_pages", GpoHeads), ("k_new", GpoHeads), ("v_new", GpoHeads),
+        ("page_table", ctypes.c_void_p), ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+def _operator(args: type) -> tuple:
+    """Signature of an operator's launch: (args, stream, log, log_cap)."""
+    return ctypes.c_int, [ctypes.POINTER(args), ctypes.c_void_p, ctypes.c_char_p,
+                          ctypes.c_size_t]
+
+
+def _workspace(args: type) -> tuple:
+    """Signature of an operator's workspace query: (args, bytes, log, log_cap)."""
+    return ctypes.c_int, [ctypes.POINTER(args), ctypes.POINTER(ctypes.c_uint64),
+                          ctypes.c_char_p, ctypes.c_size_t]
+
+
 # Every symbol include/gpo.h declares, with its ctypes signature.
 SIGNATURES = {
     "gpo_abi_version": (ctypes.c_int, []),
@@ -79,6 +123,12 @@ SIGNATURES = {
     "gpo_reduction_sum_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64,
                                                  ctypes.c_void_p, ctypes.c_int32,
                                                  ctypes.c_int32, ctypes.c_void_p]),
+    "gpo_window_attention": _operator(GpoWindowArgs),
+    "gpo_window_attention_grad": _operator(GpoWindowArgs),
+    "gpo_window_workspace": _workspace(GpoWindowArgs),
+    "gpo_paged_attention": _operator(GpoPagedArgs),
+    "gpo_paged_workspace": _workspace(GpoPagedArgs),
+    "gpo_cache_append": _operator(GpoPagedArgs),
     "gpo_destroy": (None, [ctypes.c_void_p]),
     "gpo_source": (ctypes.c_char_p, [ctypes.c_void_p]),
     "gpo_status_name": (ctypes.c_char_p, [ctypes.c_int]),

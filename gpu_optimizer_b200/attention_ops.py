@@ -1,0 +1,309 @@
+"""Window attention with sinks (forward and gradient) and paged attention.
+
+Operators for models whose attention the search tasks of this package do not
+cover: grouped heads, strided tensors, a sliding window with sink tokens, a
+gradient, and a paged K/V cache.  They run on ``libgpo.so`` (include/gpo.h)
+like the tasks do; ``runner.build_callable`` builds them too, under the names
+``attention_window``, ``attention_window_grad``, ``attention_paged`` and
+``cache_append``.
+
+* ``window_attention``            differentiable; what a training step calls
+* ``window_attention_forward``    -> (out, log-sum-exp)
+* ``window_attention_backward``   -> (dq, dk, dv)
+* ``PagedAttention``              plan of a serving loop: ``append`` writes a
+  chunk's K/V to the cache pages, ``attend`` reads them
+
+Mask: token i of a sequence with q_len new tokens and kv_len keys stands at
+p = i + kv_len - q_len and sees key j iff j <= p and (p - j < window or
+j < sinks).  A token that sees no key gives 0 and a log-sum-exp of -inf.
+
+Layouts: q, out (batch, tokens, heads_q, head_dim); k, v (batch, tokens,
+heads_kv, head_dim); heads_q a multiple of heads_kv; float16 or bfloat16;
+head_dim 64 or 128.  Any strides whose rows of head_dim are contiguous and
+16-byte aligned are read in place (slices of a fused projection, transposed
+views); others are copied first.
+
+Everything runs on torch's current stream and never synchronises.  A refused
+argument raises ``KernelBuildError`` with the library's reason, before
+anything is launched; a launch that fails raises ``RuntimeError``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .runner import KernelBuildError
+
+_DTYPE_IDS = {torch.float16: 2, torch.bfloat16: 3}
+
+
+def _library():
+    try:
+        return _lib.load()
+    except _lib.LibraryMissing as e:
+        raise KernelBuildError(str(e), log=str(e)) from e
+
+
+def _call(name: str, args, third) -> None:
+    log = ctypes.create_string_buffer(256)
+    rc = getattr(_library(), name)(args, third, log, 256)
+    if rc != _lib.OK:
+        why = log.value.decode(errors="replace")
+        text = f"{name}: {_lib.status_name(rc)}: {why}"
+        if rc in (_lib.BAD_ARGS, _lib.BAD_CONFIG):
+            raise KernelBuildError(text, log=why)
+        raise RuntimeError(text)
+
+
+def _launch(name: str, args, device: torch.device) -> None:
+    if torch.cuda.current_device() == device.index:
+        _call(name, args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _call(name, args, torch.cuda.current_stream().cuda_stream)
+
+
+def _check(name: str, t: torch.Tensor, dims: int, dtype: torch.dtype,
+           device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise KernelBuildError(f"{name} must be a CUDA tensor")
+    if t.dim() != dims:
+        raise KernelBuildError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise KernelBuildError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise KernelBuildError(f"{name} is on {t.device}, expected {device}")
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy where its rows cannot be read in place: rows that are
+    not contiguous, or a start or stride off the 16-byte grid."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        ok = ok and (n == 1 or s % 8 == 0)
+    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+
+
+def _heads(field, t: torch.Tensor) -> None:
+    """Fill a gpo_heads record from a (batch, token, head, dim) tensor, or
+    from packed (token, head, dim) rows."""
+    field.ptr = t.data_ptr()
+    s = t.stride()
+    if len(s) == 4:
+        field.stride_batch, field.stride_token, field.stride_head = s[0], s[1], s[2]
+    else:
+        field.stride_batch, field.stride_token, field.stride_head = 0, s[0], s[1]
+
+
+def _mask(args, window, sinks: int, scale) -> None:
+    if window is not None and window < 1:
+        raise KernelBuildError(f"window must be at least 1 (or None), got {window}")
+    if sinks < 0:
+        raise KernelBuildError(f"sinks must not be negative, got {sinks}")
+    if scale is not None and not scale > 0:
+        raise KernelBuildError(f"scale must be positive, got {scale}")
+    args.window = 0 if window is None else min(int(window), 1 << 40)
+    args.sinks = min(int(sinks), 1 << 40)
+    args.scale = 0.0 if scale is None else float(scale)
+
+
+def _window_args(q, k, v, window, sinks, scale):
+    if not isinstance(q, torch.Tensor) or q.dtype not in _DTYPE_IDS:
+        raise KernelBuildError("q must be a float16 or bfloat16 CUDA tensor")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(name, t, 4, q.dtype, q.device)
+    b, q_len, heads_q, dim = q.shape
+    kv_len, heads_kv = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != dim:
+        raise KernelBuildError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} "
+                               "do not belong together")
+    a = _lib.GpoWindowArgs()
+    a.dtype, a.head_dim, a.heads_q, a.heads_kv = _DTYPE_IDS[q.dtype], dim, heads_q, heads_kv
+    a.batch, a.q_len, a.kv_len = b, q_len, kv_len
+    _mask(a, window, sinks, scale)
+    _heads(a.q, q)
+    _heads(a.k, k)
+    _heads(a.v, v)
+    return a
+
+
+def window_attention_forward(q, k, v, *, window: int | None = None, sinks: int = 0,
+                             scale: float | None = None):
+    """(out, lse): attention of q over k, v, and each row's log-sum-exp of
+    scaled scores, fp32 (batch, q_len, heads_q)."""
+    q, k, v = _readable(q), _readable(k), _readable(v)
+    a = _window_args(q, k, v, window, sinks, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    _heads(a.out, out)
+    a.lse = lse.data_ptr()
+    _launch("gpo_window_attention", a, q.device)
+    return out, lse
+
+
+def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = None,
+                              sinks: int = 0, scale: float | None = None):
+    """(dq, dk, dv) from the output's gradient and what the forward returned.
+
+    Sums run in a fixed order: the same inputs give the same bits.
+    """
+    q, k, v, out, dout = (_readable(t) for t in (q, k, v, out, dout))
+    a = _window_args(q, k, v, window, sinks, scale)
+    for name, t in (("out", out), ("dout", dout)):
+        _check(name, t, 4, q.dtype, q.device)
+        if t.shape != q.shape:
+            raise KernelBuildError(f"{name} has shape {tuple(t.shape)}, expected {tuple(q.shape)}")
+    _check("lse", lse, 3, torch.float32, q.device)
+    if lse.shape != q.shape[:3]:
+        raise KernelBuildError(f"lse has shape {tuple(lse.shape)}, expected {tuple(q.shape[:3])}")
+    lse = lse.contiguous()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    for field, t in ((a.out, out), (a.dout, dout), (a.dq, dq), (a.dk, dk), (a.dv, dv)):
+        _heads(field, t)
+    a.lse = lse.data_ptr()
+    size = ctypes.c_uint64(0)
+    _call("gpo_window_workspace", a, size)
+    work = torch.empty(max(1, size.value), dtype=torch.uint8, device=q.device)
+    a.workspace, a.workspace_bytes = work.data_ptr(), size.value
+    _launch("gpo_window_attention_grad", a, q.device)
+    return dq, dk, dv
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale):
+        out, lse = window_attention_forward(q, k, v, window=window, sinks=sinks, scale=scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.mask = {"window": window, "sinks": sinks, "scale": scale}
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        return (*window_attention_backward(dout, *ctx.saved_tensors, **ctx.mask), None, None, None)
+
+
+def window_attention(q, k, v, *, window: int | None = None, sinks: int = 0,
+                     scale: float | None = None) -> torch.Tensor:
+    """Differentiable attention of q (batch, q_len, heads_q, head_dim) over
+    k, v (batch, kv_len, heads_kv, head_dim)."""
+    return _WindowAttention.apply(q, k, v, window, sinks, scale)
+
+
+class PagedAttention:
+    """Plan of attention over a paged K/V cache: fixed heads, page size, mask
+    and the most sequences and new tokens per sequence of a call.
+
+    The cache is two tensors (num_pages, page_size, heads_kv, head_dim).
+    Per call, ``page_table`` (int32, seqs x width) names the page of every
+    ``page_size`` slots of a sequence, ``q_start`` (int32, seqs + 1) the first
+    row of each sequence in the packed rows, and ``kv_len`` (int32, seqs) its
+    keys, new tokens included.  Both stay on the device and are not read by
+    the host; a sequence whose lengths do not fit the buffers is skipped and
+    reported by ``runner.check_device_status``.  Page table entries behind a
+    sequence's last key, and those of pages no token sees any more, are not
+    read as pages.
+
+    The plan owns the kernels' workspace: calls of one plan have to follow
+    one another on a stream; concurrent streams need a plan each.
+    """
+
+    def __init__(self, *, heads_q: int, heads_kv: int, head_dim: int, page_size: int,
+                 max_seqs: int, max_q: int, dtype: torch.dtype, window: int | None = None,
+                 sinks: int = 0, scale: float | None = None, device=None) -> None:
+        if dtype not in _DTYPE_IDS:
+            raise KernelBuildError(f"dtype must be float16 or bfloat16, got {dtype}")
+        if max_seqs < 1 or max_q < 1:
+            raise KernelBuildError("max_seqs and max_q must be at least 1")
+        self.dtype, self.heads_q, self.heads_kv, self.head_dim = dtype, heads_q, heads_kv, head_dim
+        self.page_size, self.max_seqs, self.max_q = page_size, max_seqs, max_q
+        device = torch.device("cuda" if device is None else device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        a = self._args = _lib.GpoPagedArgs()
+        a.dtype, a.head_dim, a.heads_q, a.heads_kv = _DTYPE_IDS[dtype], head_dim, heads_q, heads_kv
+        a.page_size, a.max_q = page_size, max_q
+        _mask(a, window, sinks, scale)
+        a.num_seqs, a.tokens = max_seqs, max_seqs * max_q
+        size = ctypes.c_uint64(0)
+        _call("gpo_paged_workspace", a, size)
+        self._work = torch.zeros(max(1, size.value), dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = self._work.data_ptr(), size.value
+
+    def _fill(self, rows, k_pages, v_pages, page_table, q_start, kv_len):
+        a = self._args
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _check(name, t, 4, self.dtype, self.device)
+            if t.shape[1:] != (self.page_size, self.heads_kv, self.head_dim):
+                raise KernelBuildError(
+                    f"{name} has shape {tuple(t.shape)}, expected (pages, {self.page_size}, "
+                    f"{self.heads_kv}, {self.head_dim})")
+            if t.stride(3) != 1:
+                raise KernelBuildError(f"{name}: rows must be contiguous")
+        if k_pages.shape[0] != v_pages.shape[0]:
+            raise KernelBuildError("k_pages and v_pages have different numbers of pages")
+        _check("page_table", page_table, 2, torch.int32, self.device)
+        _check("q_start", q_start, 1, torch.int32, self.device)
+        _check("kv_len", kv_len, 1, torch.int32, self.device)
+        seqs, width = page_table.shape
+        if seqs > self.max_seqs or q_start.shape[0] != seqs + 1 or kv_len.shape[0] != seqs:
+            raise KernelBuildError(
+                f"{seqs} sequences in page_table, {q_start.shape[0] - 1} in q_start, "
+                f"{kv_len.shape[0]} in kv_len; at most {self.max_seqs}")
+        if (width > 1 and page_table.stride(1) != 1) or not q_start.is_contiguous() \
+                or not kv_len.is_contiguous():
+            raise KernelBuildError("page_table rows, q_start and kv_len must be contiguous")
+        a.num_seqs, a.tokens, a.num_pages = seqs, rows, k_pages.shape[0]
+        a.table_width, a.table_stride = width, page_table.stride(0)
+        a.page_table, a.q_start, a.kv_len = (page_table.data_ptr(), q_start.data_ptr(),
+                                             kv_len.data_ptr())
+        _heads(a.k_pages, k_pages)
+        _heads(a.v_pages, v_pages)
+        return a
+
+    def append(self, k, v, k_pages, v_pages, page_table, q_start, kv_len) -> None:
+        """Write the new tokens' rows k, v (tokens, heads_kv, head_dim) to the
+        last slots of their sequences: token i to kv_len - q_len + i."""
+        for name, t in (("k", k), ("v", v)):
+            _check(name, t, 3, self.dtype, self.device)
+            if t.shape[1:] != (self.heads_kv, self.head_dim) or t.shape[0] != k.shape[0]:
+                raise KernelBuildError(f"{name} has shape {tuple(t.shape)}, expected (tokens, "
+                                       f"{self.heads_kv}, {self.head_dim})")
+        k, v = _readable(k), _readable(v)
+        a = self._fill(k.shape[0], k_pages, v_pages, page_table, q_start, kv_len)
+        _heads(a.k_new, k)
+        _heads(a.v_new, v)
+        _launch("gpo_cache_append", a, self.device)
+
+    def attend(self, q, k_pages, v_pages, page_table, q_start, kv_len, out=None,
+               lse=None) -> torch.Tensor:
+        """Attention of the new tokens q (tokens, heads_q, head_dim) over
+        their sequences' pages; the tokens' own K/V are in the cache already.
+        ``out`` may name the tensor to write, ``lse`` (fp32, tokens x heads_q)
+        one for the log-sum-exp."""
+        _check("q", q, 3, self.dtype, self.device)
+        if q.shape[1:] != (self.heads_q, self.head_dim):
+            raise KernelBuildError(f"q has shape {tuple(q.shape)}, expected (tokens, "
+                                   f"{self.heads_q}, {self.head_dim})")
+        q = _readable(q)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _check("out", out, 3, self.dtype, self.device)
+            if out.shape != q.shape or out.stride(2) != 1:
+                raise KernelBuildError(f"out must be like q {tuple(q.shape)}, rows contiguous")
+        if lse is not None:
+            _check("lse", lse, 2, torch.float32, self.device)
+            if lse.shape != q.shape[:2] or not lse.is_contiguous():
+                raise KernelBuildError(f"lse must be a contiguous {tuple(q.shape[:2])} tensor")
+        a = self._fill(q.shape[0], k_pages, v_pages, page_table, q_start, kv_len)
+        _heads(a.q, q)
+        _heads(a.out, out)
+        a.lse = 0 if lse is None else lse.data_ptr()
+        _launch("gpo_paged_attention", a, self.device)
+        return out

@@ -25,6 +25,7 @@ CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libgpo.so"
 HEADERS = [CSRC / "gpo_common.cuh", CSRC / "gpo_internal.h", ROOT / "include" / "gpo.h"]
+OPS_HEADER = CSRC / "attn_ops.cuh"  # of the *_ops.cu units and ops_abi.cu
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -78,7 +79,8 @@ def build(jobs: int | None = None, verbose: bool = False, force: bool = False) -
     for s in srcs:
         o = BUILD / (s.stem + ".o")
         objs.append(o)
-        deps = HEADERS + ([inc] if s.stem == "abi" else [])
+        deps = (HEADERS + ([inc] if s.stem == "abi" else [])
+                + ([OPS_HEADER] if "ops" in s.stem else []))
         if force or _stale(o, s, deps):
             todo.append((s, o))
 

@@ -95,6 +95,8 @@ const char* family_source(const std::string& family) {
   return nullptr;
 }
 
+}  // namespace
+
 void write_log(char* log, size_t cap, const std::string& msg) {
   if (!log || cap == 0) return;
   const size_t n = msg.size() < cap - 1 ? msg.size() : cap - 1;
@@ -102,7 +104,18 @@ void write_log(char* log, size_t cap, const std::string& msg) {
   log[n] = '\0';
 }
 
-}  // namespace
+gpo_status launch_ctx(void* stream, LaunchCtx* out) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return GPO_NO_DEVICE;
+  }
+  DeviceState* ds = nullptr;
+  const gpo_status s = device_state(dev, &ds);
+  if (s != GPO_OK) return s;
+  *out = LaunchCtx{static_cast<cudaStream_t>(stream), ds->err, dev, ds->sm_count};
+  return GPO_OK;
+}
 
 gpo_status ensure_smem_attr(const void* func, uint32_t dyn_smem) {
   if (dyn_smem <= 48u * 1024u) return GPO_OK;

@@ -1,0 +1,168 @@
+// What the window / paged attention kernels share: which keys a tile of
+// query rows sees, tensor maps over strided heads, and the launch records.
+//
+// Heads are grouped: query head h reads kv head h / g.  A tile of query rows
+// packs all g query heads of one kv head: row r of a tile that starts at
+// token t0 is token t0 + r / g, head r % g, so one K/V block serves g heads
+// from a single shared-memory copy.  A tile holds tpt = 128 / g whole tokens
+// (rows tpt * g .. 127 are unused when g does not divide 128).
+//
+// Mask: token i of a sequence with q_len new tokens and kv_len keys stands
+// at p = i + kv_len - q_len and sees key j iff j <= p and
+// (p - j < window or j < sinks).
+#pragma once
+
+#include "gpo_common.cuh"
+#include "gpo_internal.h"
+
+namespace gpo {
+
+constexpr int kOpsBN = 128;              // keys per block
+constexpr int kOpsNoWindow = 1 << 30;    // a window that reaches every key
+constexpr int kOpsMaxLen = 1 << 30;      // largest q_len / kv_len
+
+// The part of a problem that every role of a kernel needs.
+struct AttnGeom {
+  const int* q_start;   // paged: first row of each sequence (batch + 1 values)
+  const int* kv_lens;   // paged: keys of each sequence, its new tokens included
+  const int* table;     // paged: page of every page_size slots
+  int64_t table_stride;
+  int table_width;
+  int page_size, box_rows, num_pages;
+  int batch, q_len, kv_len;  // q_len: dense length, or the most a sequence has
+  int tokens;                // paged: rows of q
+  int heads_kv, g, tpt;
+  int tiles;                 // query tiles per sequence (of the longest one)
+  int window, sinks;
+};
+
+struct AttnSeq {
+  int q_len, kv_len;
+  int row0;  // first row of the sequence in the packed q (paged), else 0
+  int off;   // position of token 0
+};
+
+// Lengths of sequence b.  Paged lengths are device data that the host has
+// not seen: values that do not fit the buffers are cut to what does.
+template <bool PAGED>
+__device__ __forceinline__ AttnSeq attn_seq(const AttnGeom& g, int b, unsigned int* err) {
+  AttnSeq s;
+  if constexpr (PAGED) {
+    const int a = __ldg(g.q_start + b), e = __ldg(g.q_start + b + 1);
+    const int n = __ldg(g.kv_lens + b);
+    const int64_t cap = static_cast<int64_t>(g.table_width) * g.page_size;
+    s.row0 = a;
+    s.q_len = e - a;
+    s.kv_len = n;
+    if (a < 0 || e < a || e > g.tokens || s.q_len > g.q_len || n < 0 || n > cap) {
+      s.row0 = 0;
+      s.q_len = 0;
+      s.kv_len = 0;
+      if (threadIdx.x == 0) atomicOr(err, kErrBadLaunch);
+    }
+  } else {
+    s.row0 = 0;
+    s.q_len = g.q_len;
+    s.kv_len = g.kv_len;
+  }
+  s.off = s.kv_len - s.q_len;
+  return s;
+}
+
+// K/V blocks that some row of tokens [t0, t1) sees: the sink blocks
+// [0, sink_blocks) and then the blocks first, first + 1, ... of the window.
+struct AttnBlocks {
+  int n, sink_blocks, first;
+  __device__ __forceinline__ int at(int i) const {
+    return i < sink_blocks ? i : first + i - sink_blocks;
+  }
+};
+
+__device__ __forceinline__ AttnBlocks attn_blocks(const AttnGeom& g, const AttnSeq& s, int t0,
+                                                  int t1) {
+  AttnBlocks b{0, 0, 0};
+  const int hi = t1 - 1 + s.off;  // last position: the last key any row sees
+  if (t0 >= t1 || hi < 0) return b;
+  const int lo = max(0, t0 + s.off - g.window + 1);
+  b.first = lo / kOpsBN;
+  b.sink_blocks = min(b.first, (min(g.sinks, hi + 1) + kOpsBN - 1) / kOpsBN);
+  b.n = b.sink_blocks + hi / kOpsBN - b.first + 1;
+  return b;
+}
+
+// Keys of a block that a row at position p sees: i <= hi and
+// (i >= lo or i < sink), i counted from the block's first key.
+struct RowMask {
+  int hi, lo, sink;
+  __device__ __forceinline__ bool sees(int i) const { return i <= hi && (i >= lo || i < sink); }
+};
+
+__device__ __forceinline__ RowMask row_mask(const AttnGeom& g, int p, int key0) {
+  return RowMask{p - key0, p - g.window + 1 - key0, g.sinks - key0};
+}
+
+// Whether some row of tokens [t0, t1) misses a key of the block.
+__device__ __forceinline__ bool block_is_masked(const AttnGeom& g, const AttnSeq& s, int t0,
+                                                int t1, int key0) {
+  return key0 + kOpsBN - 1 > t0 + s.off || (t1 - 1 + s.off - g.window + 1 > key0 &&
+                                            key0 + kOpsBN > g.sinks);
+}
+
+// 5-D tiled load (see tma_load_3d).
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t x, int32_t y, int32_t z, int32_t u,
+                                            int32_t v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t x, int32_t y, int32_t z, int32_t u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+
+// ------------------------------------------------------------------- host
+// One strided (batch, token, head, dim) tensor of 16-bit elements.
+struct HeadsView {
+  const void* ptr;
+  int64_t batch, tokens, heads;
+  int64_t s_batch, s_token, s_head;  // elements
+};
+
+// Tile of a query-side tensor: {64 dims, g heads, 1 kv head, tpt tokens}.
+bool encode_rows_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, int g, int tpt);
+// Block of a key-side tensor: {64 dims, 1 head, rows, 1 batch or page}.
+bool encode_keys_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, int rows);
+
+// A checked problem, as the entry points hand it to the launchers.
+struct AttnProblem {
+  AttnGeom geom;
+  int dtype, dim;
+  bool paged;
+  float scale;
+  HeadsView q, k, v;         // paged: k and v are the pages
+  HeadsView k_new, v_new;    // append
+  void* out;
+  int64_t o_batch, o_token, o_head;
+  float* lse;
+};
+
+// What the gradient adds to a dense problem.
+struct AttnGradProblem {
+  HeadsView out, dout, dq, dk, dv;
+  const float* lse;
+  void* workspace;
+};
+
+uint64_t attn_grad_workspace(const AttnProblem& p);
+gpo_status launch_attn_grad(const AttnProblem& p, const AttnGradProblem& gp, const LaunchCtx& c);
+gpo_status launch_attn_forward(const AttnProblem& p, const LaunchCtx& c);
+gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c);
+
+}  // namespace gpo

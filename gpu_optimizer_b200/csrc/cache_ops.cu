@@ -1,0 +1,77 @@
+// Append of new tokens' K/V rows to a paged cache: a copy with a gather of
+// addresses.  Its floor is the rows' bytes, read and written once; for a
+// few tokens a launch.  One thread moves one 16-byte vector of a row of K
+// and of V; the token's sequence is found by a binary search of q_start,
+// whose values every thread of a block reads from the same cache lines.
+#include "attn_ops.cuh"
+
+namespace gpo {
+
+struct AppendArgs {
+  AttnGeom geom;
+  const uint4 *k_new, *v_new;
+  uint4 *k_pages, *v_pages;
+  // in 16-byte vectors
+  int64_t kn_token, kn_head, vn_token, vn_head;
+  int64_t kp_page, kp_slot, kp_head, vp_page, vp_slot, vp_head;
+  int vecs;  // vectors of a row
+};
+
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+  const AttnGeom& g = a.geom;
+  const int per_token = g.heads_kv * a.vecs;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t t64 = i / per_token;
+  if (t64 >= g.tokens) return;
+  const int t = static_cast<int>(t64);
+  const int e = static_cast<int>(i - t64 * per_token);
+  const int h = e / a.vecs, x = e % a.vecs;
+  // the sequence b with q_start[b] <= t < q_start[b + 1]
+  int lo = 0, hi = g.batch;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (__ldg(g.q_start + m) <= t)
+      lo = m;
+    else
+      hi = m;
+  }
+  const int first = __ldg(g.q_start + lo), end = __ldg(g.q_start + lo + 1);
+  if (t < first || t >= end) return;
+  const int64_t slot = static_cast<int64_t>(__ldg(g.kv_lens + lo)) - (end - t);
+  const int64_t at = slot / g.page_size;
+  if (slot < 0 || at >= g.table_width) return;
+  const int page = __ldg(g.table + lo * g.table_stride + at);
+  if (page < 0 || page >= g.num_pages) return;
+  const int64_t s = slot - at * g.page_size;
+  const uint4 kv = __ldcs(a.k_new + t * a.kn_token + h * a.kn_head + x);
+  const uint4 vv = __ldcs(a.v_new + t * a.vn_token + h * a.vn_head + x);
+  a.k_pages[page * a.kp_page + s * a.kp_slot + h * a.kp_head + x] = kv;
+  a.v_pages[page * a.vp_page + s * a.vp_slot + h * a.vp_head + x] = vv;
+}
+
+gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c) {
+  AppendArgs a;
+  a.geom = p.geom;
+  a.k_new = static_cast<const uint4*>(p.k_new.ptr);
+  a.v_new = static_cast<const uint4*>(p.v_new.ptr);
+  a.k_pages = static_cast<uint4*>(const_cast<void*>(p.k.ptr));
+  a.v_pages = static_cast<uint4*>(const_cast<void*>(p.v.ptr));
+  a.kn_token = p.k_new.s_token / 8;
+  a.kn_head = p.k_new.s_head / 8;
+  a.vn_token = p.v_new.s_token / 8;
+  a.vn_head = p.v_new.s_head / 8;
+  a.kp_page = p.k.s_batch / 8;
+  a.kp_slot = p.k.s_token / 8;
+  a.kp_head = p.k.s_head / 8;
+  a.vp_page = p.v.s_batch / 8;
+  a.vp_slot = p.v.s_token / 8;
+  a.vp_head = p.v.s_head / 8;
+  a.vecs = p.dim / 8;
+  const uint64_t n = static_cast<uint64_t>(p.geom.tokens) * p.geom.heads_kv * a.vecs;
+  const uint64_t blocks = cdiv(n, 256);
+  if (blocks > 0x7fffffffull) return GPO_BAD_ARGS;
+  cache_append_kernel<<<static_cast<unsigned>(blocks), 256, 0, c.stream>>>(a);
+  return launch_status();
+}
+
+}  // namespace gpo

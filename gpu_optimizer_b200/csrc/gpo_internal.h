@@ -82,6 +82,13 @@ inline gpo_status launch_status() {
 // Set the dynamic shared memory opt-in of a kernel once per device.
 gpo_status ensure_smem_attr(const void* func, uint32_t dyn_smem);
 
+// Launch context of the current device for `stream` (allocates the device's
+// error word on first use).
+gpo_status launch_ctx(void* stream, LaunchCtx* out);
+
+// Copy a message into a caller's log buffer (cut to fit, may be null).
+void write_log(char* log, size_t cap, const std::string& msg);
+
 // Grid of a persistent kernel: SM count x resident CTAs per SM (occupancy
 // of `func` at `threads` / `dyn_smem`, cached), at most `work_items`.
 unsigned persistent_grid(const void* func, int threads, size_t dyn_smem, int sm_count,

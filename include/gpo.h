@@ -201,6 +201,105 @@ GPO_API gpo_status gpo_reduction_sum_noalloc(const float* x, int64_t n, float* o
                                              int32_t block_size, int32_t num_warps,
                                              void* stream);
 
+/* ------------------------------------------------ window / paged attention
+ * Attention with a sliding window and sink tokens over grouped heads:
+ * a dense form with its gradient (training), and a form that reads a paged
+ * K/V cache (serving: chunks of new tokens, single tokens included), with
+ * the call that writes the cache.  No counterpart in the reference.
+ *
+ * Mask of all of them: token i of a sequence with q_len new tokens and
+ * kv_len keys stands at position p = i + kv_len - q_len and sees key j iff
+ * j <= p and (p - j < window or j < sinks).  A row that sees no key gives 0
+ * and a log-sum-exp of -inf.  What a masked place holds (NaN and infinities
+ * included) does not reach the scores; the values that a masked key weighs
+ * with 0 have to be finite wherever another row of the sequence sees it.
+ *
+ * Query head h reads kv head h / (heads_q / heads_kv).  Element types:
+ * GPO_FLOAT16 or GPO_BFLOAT16, fp32 scores, statistics and sums.
+ * head_dim: 64 or 128.  Every row of head_dim elements is contiguous and
+ * 16-byte aligned (strides are in elements, multiples of 8).
+ *
+ * Arguments are checked before anything is launched; on a refusal a
+ * readable reason is written to `log` (which may be NULL). */
+
+/* A strided (batch, token, head, head_dim) tensor; paged caches: batch is
+ * the page, token the slot in it; packed rows: stride_batch is unused. */
+typedef struct gpo_heads {
+  void* ptr;
+  int64_t stride_batch, stride_token, stride_head;
+} gpo_heads;
+
+typedef struct gpo_window_args {
+  int32_t dtype, head_dim, heads_q, heads_kv;
+  int64_t batch, q_len, kv_len;
+  int64_t window;      /* keys a query sees, its own included; 0: no window */
+  int64_t sinks;       /* first keys that stay visible                      */
+  float scale;         /* of the scores; 0: 1 / sqrt(head_dim)              */
+  int32_t reserved;    /* 0 */
+  gpo_heads q, k, v;   /* inputs                                            */
+  gpo_heads out;       /* forward: written; backward: read                  */
+  float* lse;          /* (batch, q_len, heads_q) fp32; forward: written
+                          unless NULL; backward: read                       */
+  gpo_heads dout;      /* backward: gradient of out                         */
+  gpo_heads dq, dk, dv; /* backward: written                                */
+  void* workspace;     /* backward: gpo_window_workspace bytes, 256-aligned */
+  uint64_t workspace_bytes;
+} gpo_window_args;
+
+typedef struct gpo_paged_args {
+  int32_t dtype, head_dim, heads_q, heads_kv;
+  int64_t num_seqs;
+  int64_t tokens;      /* rows of q (and of k_new, v_new)                   */
+  int64_t max_q;       /* at least the most new tokens of any sequence      */
+  int64_t num_pages;
+  int64_t page_size;   /* slots of a page: a multiple of 8                  */
+  int64_t table_width; /* pages per sequence in page_table                  */
+  int64_t table_stride; /* elements between its rows                        */
+  int64_t window, sinks;
+  float scale;
+  int32_t reserved;    /* 0 */
+  gpo_heads q, out;    /* packed rows (token, head)                         */
+  gpo_heads k_pages, v_pages;
+  gpo_heads k_new, v_new; /* gpo_cache_append: the new tokens' rows         */
+  const int32_t* page_table; /* device: page of each page_size slots        */
+  const int32_t* q_start;    /* device: first row of each sequence, then
+                                tokens (num_seqs + 1 values, ascending)     */
+  const int32_t* kv_len;     /* device: keys of each sequence, its new
+                                tokens included                             */
+  float* lse;          /* (tokens, heads_q) fp32 or NULL                    */
+  void* workspace;     /* gpo_paged_workspace bytes, 256-aligned, zeroed
+                          once by the caller; calls that may overlap need
+                          one each                                          */
+  uint64_t workspace_bytes;
+} gpo_paged_args;
+
+/* Dense forward: out and lse. */
+GPO_API gpo_status gpo_window_attention(const gpo_window_args* args, void* stream, char* log,
+                                        size_t log_cap);
+/* Gradients dq, dk, dv from dout, the inputs and the forward's out and lse.
+ * Sums are taken in a fixed order: equal inputs give equal bits. */
+GPO_API gpo_status gpo_window_attention_grad(const gpo_window_args* args, void* stream, char* log,
+                                             size_t log_cap);
+/* Bytes of workspace that gpo_window_attention_grad needs for `args` (its
+ * pointers are not looked at). */
+GPO_API gpo_status gpo_window_workspace(const gpo_window_args* args, uint64_t* bytes, char* log,
+                                        size_t log_cap);
+
+/* Attention of each sequence's new tokens (rows q_start[b] .. q_start[b+1])
+ * over its cache pages, which hold the new tokens' K/V already.  Lengths
+ * and pages stay on the device: a sequence whose lengths do not fit the
+ * buffers is skipped (its rows of out are not written) and reported by
+ * gpo_device_status (bit 5); a page outside [0, num_pages) reads as zeros. */
+GPO_API gpo_status gpo_paged_attention(const gpo_paged_args* args, void* stream, char* log,
+                                       size_t log_cap);
+GPO_API gpo_status gpo_paged_workspace(const gpo_paged_args* args, uint64_t* bytes, char* log,
+                                       size_t log_cap);
+/* Write the new tokens' rows k_new, v_new to the last slots of their
+ * sequences: token i to slot kv_len - q_len + i.  Rows whose slot or page is
+ * outside the buffers are not written. */
+GPO_API gpo_status gpo_cache_append(const gpo_paged_args* args, void* stream, char* log,
+                                    size_t log_cap);
+
 /* Free a module. */
 GPO_API void gpo_destroy(gpo_module* mod);
 
