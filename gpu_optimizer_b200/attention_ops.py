@@ -31,13 +31,26 @@ anything is launched; a launch that fails raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _lib
 from .runner import KernelBuildError
 
-_DTYPE_IDS = {torch.float16: 2, torch.bfloat16: 3}
+_DTYPE_IDS = {torch.float16: _lib.DTYPE_IDS["float16"], torch.bfloat16: _lib.DTYPE_IDS["bfloat16"]}
+
+# A call's records are packed in one go: field by field costs more than the
+# launch.  (ptr, stride_batch, stride_token, stride_head) per tensor.
+_HEADS = "Q3q"
+_WINDOW = struct.Struct("<4i5qfi" + 4 * _HEADS + "Q" + 4 * _HEADS + "QQ")
+_NO_HEADS = (0, 0, 0, 0)
+_PAGED_SIZES = struct.Struct("<qq")             # num_seqs, tokens
+_PAGED_PAGES = struct.Struct("<q")              # num_pages
+_PAGED_TABLE = struct.Struct("<qq")             # table_width, table_stride
+_PAGED_HEADS = struct.Struct("<" + 2 * _HEADS)  # q, out / k_pages, v_pages / k_new, v_new
+_PAGED_PTRS = struct.Struct("<4Q")              # page_table, q_start, kv_len, lse
+assert _WINDOW.size == ctypes.sizeof(_lib.GpoWindowArgs)
 
 
 def _library():
@@ -47,23 +60,35 @@ def _library():
         raise KernelBuildError(str(e), log=str(e)) from e
 
 
-def _call(name: str, args, third) -> None:
-    log = ctypes.create_string_buffer(256)
-    rc = getattr(_library(), name)(args, third, log, 256)
-    if rc != _lib.OK:
-        why = log.value.decode(errors="replace")
-        text = f"{name}: {_lib.status_name(rc)}: {why}"
-        if rc in (_lib.BAD_ARGS, _lib.BAD_CONFIG):
-            raise KernelBuildError(text, log=why)
-        raise RuntimeError(text)
+def _refused(name: str, rc: int, log) -> None:
+    why = log.value.decode(errors="replace")
+    text = f"{name}: {_lib.status_name(rc)}: {why}"
+    if rc in (_lib.BAD_ARGS, _lib.BAD_CONFIG):
+        raise KernelBuildError(text, log=why)
+    raise RuntimeError(text)
 
 
 def _launch(name: str, args, device: torch.device) -> None:
-    if torch.cuda.current_device() == device.index:
-        _call(name, args, torch.cuda.current_stream().cuda_stream)
+    """Call a launch entry point on ``device``'s current torch stream."""
+    fn = getattr(_library(), name)
+    index = device.index
+    log = ctypes.create_string_buffer(256)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index), log, 256)
     else:
-        with torch.cuda.device(device):
-            _call(name, args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index), log, 256)
+    if rc != _lib.OK:
+        _refused(name, rc, log)
+
+
+def _workspace_bytes(name: str, args) -> int:
+    log = ctypes.create_string_buffer(256)
+    size = ctypes.c_uint64(0)
+    rc = getattr(_library(), name)(args, size, log, 256)
+    if rc != _lib.OK:
+        _refused(name, rc, log)
+    return size.value
 
 
 def _check(name: str, t: torch.Tensor, dims: int, dtype: torch.dtype,
@@ -72,61 +97,70 @@ def _check(name: str, t: torch.Tensor, dims: int, dtype: torch.dtype,
         raise KernelBuildError(f"{name} must be a CUDA tensor")
     if t.dim() != dims:
         raise KernelBuildError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise KernelBuildError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise KernelBuildError(f"{name} is on {t.device}, expected {device}")
 
 
+def _in_place(t: torch.Tensor) -> bool:
+    """Whether the kernels can address ``t``'s rows where they are."""
+    *steps, last = t.stride()
+    if last == 1 and t.data_ptr() & 15 == 0:
+        if all(s & 7 == 0 for s in steps):
+            return True
+        return all(s & 7 == 0 for n, s in zip(t.shape, steps) if n > 1)
+    return t.numel() == 0
+
+
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """``t``, or a copy where its rows cannot be read in place: rows that are
     not contiguous, or a start or stride off the 16-byte grid."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
-        ok = ok and (n == 1 or s % 8 == 0)
-    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    return t if _in_place(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _heads(field, t: torch.Tensor) -> None:
-    """Fill a gpo_heads record from a (batch, token, head, dim) tensor, or
-    from packed (token, head, dim) rows."""
-    field.ptr = t.data_ptr()
+def _heads(t: torch.Tensor) -> tuple:
+    """gpo_heads fields of a (batch, token, head, dim) tensor, or of packed
+    (token, head, dim) rows."""
     s = t.stride()
     if len(s) == 4:
-        field.stride_batch, field.stride_token, field.stride_head = s[0], s[1], s[2]
-    else:
-        field.stride_batch, field.stride_token, field.stride_head = 0, s[0], s[1]
+        return t.data_ptr(), s[0], s[1], s[2]
+    return t.data_ptr(), 0, s[0], s[1]
 
 
-def _mask(args, window, sinks: int, scale) -> None:
+def _mask(window, sinks: int, scale) -> tuple:
+    """window, sinks and scale fields."""
     if window is not None and window < 1:
         raise KernelBuildError(f"window must be at least 1 (or None), got {window}")
     if sinks < 0:
         raise KernelBuildError(f"sinks must not be negative, got {sinks}")
     if scale is not None and not scale > 0:
         raise KernelBuildError(f"scale must be positive, got {scale}")
-    args.window = 0 if window is None else min(int(window), 1 << 40)
-    args.sinks = min(int(sinks), 1 << 40)
-    args.scale = 0.0 if scale is None else float(scale)
+    return (0 if window is None else min(int(window), 1 << 40), min(int(sinks), 1 << 40),
+            0.0 if scale is None else float(scale))
 
 
-def _window_args(q, k, v, window, sinks, scale):
+def _window_sizes(q, k, v, window, sinks, scale) -> tuple:
+    """Leading fields of a gpo_window_args, after checks of q, k and v."""
     if not isinstance(q, torch.Tensor) or q.dtype not in _DTYPE_IDS:
         raise KernelBuildError("q must be a float16 or bfloat16 CUDA tensor")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check(name, t, 4, q.dtype, q.device)
+    dtype, device = q.dtype, q.device
+    _check("q", q, 4, dtype, device)
+    _check("k", k, 4, dtype, device)
+    _check("v", v, 4, dtype, device)
     b, q_len, heads_q, dim = q.shape
-    kv_len, heads_kv = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != dim:
+    kb, kv_len, heads_kv, kdim = ks = k.shape
+    if ks != v.shape or kb != b or kdim != dim:
         raise KernelBuildError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} "
                                "do not belong together")
+    return (_DTYPE_IDS[dtype], dim, heads_q, heads_kv, b, q_len, kv_len,
+            *_mask(window, sinks, scale), 0)
+
+
+def _window_args(sizes, q, k, v, out, lse, grads=4 * _NO_HEADS, workspace=(0, 0)):
     a = _lib.GpoWindowArgs()
-    a.dtype, a.head_dim, a.heads_q, a.heads_kv = _DTYPE_IDS[q.dtype], dim, heads_q, heads_kv
-    a.batch, a.q_len, a.kv_len = b, q_len, kv_len
-    _mask(a, window, sinks, scale)
-    _heads(a.q, q)
-    _heads(a.k, k)
-    _heads(a.v, v)
+    _WINDOW.pack_into(a, 0, *sizes, *_heads(q), *_heads(k), *_heads(v), *_heads(out),
+                      lse.data_ptr(), *grads, *workspace)
     return a
 
 
@@ -134,13 +168,11 @@ def window_attention_forward(q, k, v, *, window: int | None = None, sinks: int =
                              scale: float | None = None):
     """(out, lse): attention of q over k, v, and each row's log-sum-exp of
     scaled scores, fp32 (batch, q_len, heads_q)."""
+    sizes = _window_sizes(q, k, v, window, sinks, scale)
     q, k, v = _readable(q), _readable(k), _readable(v)
-    a = _window_args(q, k, v, window, sinks, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    _heads(a.out, out)
-    a.lse = lse.data_ptr()
-    _launch("gpo_window_attention", a, q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    _launch("gpo_window_attention", _window_args(sizes, q, k, v, out, lse), q.device)
     return out, lse
 
 
@@ -150,27 +182,24 @@ def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = N
 
     Sums run in a fixed order: the same inputs give the same bits.
     """
-    q, k, v, out, dout = (_readable(t) for t in (q, k, v, out, dout))
-    a = _window_args(q, k, v, window, sinks, scale)
+    sizes = _window_sizes(q, k, v, window, sinks, scale)
+    shape, device = q.shape, q.device
     for name, t in (("out", out), ("dout", dout)):
-        _check(name, t, 4, q.dtype, q.device)
-        if t.shape != q.shape:
-            raise KernelBuildError(f"{name} has shape {tuple(t.shape)}, expected {tuple(q.shape)}")
-    _check("lse", lse, 3, torch.float32, q.device)
-    if lse.shape != q.shape[:3]:
-        raise KernelBuildError(f"lse has shape {tuple(lse.shape)}, expected {tuple(q.shape[:3])}")
+        _check(name, t, 4, q.dtype, device)
+        if t.shape != shape:
+            raise KernelBuildError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    _check("lse", lse, 3, torch.float32, device)
+    if lse.shape != shape[:3]:
+        raise KernelBuildError(f"lse has shape {tuple(lse.shape)}, expected {tuple(shape[:3])}")
+    q, k, v, out, dout = (_readable(q), _readable(k), _readable(v), _readable(out),
+                          _readable(dout))
     lse = lse.contiguous()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    for field, t in ((a.out, out), (a.dout, dout), (a.dq, dq), (a.dk, dk), (a.dv, dv)):
-        _heads(field, t)
-    a.lse = lse.data_ptr()
-    size = ctypes.c_uint64(0)
-    _call("gpo_window_workspace", a, size)
-    work = torch.empty(max(1, size.value), dtype=torch.uint8, device=q.device)
-    a.workspace, a.workspace_bytes = work.data_ptr(), size.value
-    _launch("gpo_window_attention_grad", a, q.device)
+    dq, dk, dv = q.new_empty(shape), q.new_empty(k.shape), q.new_empty(k.shape)
+    grads = (*_heads(dout), *_heads(dq), *_heads(dk), *_heads(dv))
+    size = _workspace_bytes("gpo_window_workspace", _window_args(sizes, q, k, v, out, lse))
+    work = torch.empty(max(1, size), dtype=torch.uint8, device=device)
+    a = _window_args(sizes, q, k, v, out, lse, grads, (work.data_ptr(), size))
+    _launch("gpo_window_attention_grad", a, device)
     return dq, dk, dv
 
 
@@ -225,45 +254,47 @@ class PagedAttention:
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
-        a = self._args = _lib.GpoPagedArgs()
-        a.dtype, a.head_dim, a.heads_q, a.heads_kv = _DTYPE_IDS[dtype], head_dim, heads_q, heads_kv
-        a.page_size, a.max_q = page_size, max_q
-        _mask(a, window, sinks, scale)
-        a.num_seqs, a.tokens = max_seqs, max_seqs * max_q
-        size = ctypes.c_uint64(0)
-        _call("gpo_paged_workspace", a, size)
-        self._work = torch.zeros(max(1, size.value), dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = self._work.data_ptr(), size.value
+        win, sink, factor = _mask(window, sinks, scale)
+        a = self._args = _lib.GpoPagedArgs(
+            dtype=_DTYPE_IDS[dtype], head_dim=head_dim, heads_q=heads_q, heads_kv=heads_kv,
+            page_size=page_size, max_q=max_q, window=win, sinks=sink, scale=factor,
+            num_seqs=max_seqs, tokens=max_seqs * max_q)
+        size = _workspace_bytes("gpo_paged_workspace", a)
+        self._work = torch.zeros(max(1, size), dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = self._work.data_ptr(), size
+        self._page_shape = (page_size, heads_kv, head_dim)
 
-    def _fill(self, rows, k_pages, v_pages, page_table, q_start, kv_len):
-        a = self._args
+    def _fill(self, rows, k_pages, v_pages, page_table, q_start, kv_len, lse=0):
+        a, dtype, device = self._args, self.dtype, self.device
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            _check(name, t, 4, self.dtype, self.device)
-            if t.shape[1:] != (self.page_size, self.heads_kv, self.head_dim):
-                raise KernelBuildError(
-                    f"{name} has shape {tuple(t.shape)}, expected (pages, {self.page_size}, "
-                    f"{self.heads_kv}, {self.head_dim})")
-            if t.stride(3) != 1:
-                raise KernelBuildError(f"{name}: rows must be contiguous")
-        if k_pages.shape[0] != v_pages.shape[0]:
+            _check(name, t, 4, dtype, device)
+            if t.shape[1:] != self._page_shape:
+                raise KernelBuildError(f"{name} has shape {tuple(t.shape)}, expected (pages, "
+                                       f"{', '.join(map(str, self._page_shape))})")
+            if not _in_place(t):
+                raise KernelBuildError(f"{name}: rows must be contiguous and 16-byte aligned")
+        pages = k_pages.shape[0]
+        if pages != v_pages.shape[0]:
             raise KernelBuildError("k_pages and v_pages have different numbers of pages")
-        _check("page_table", page_table, 2, torch.int32, self.device)
-        _check("q_start", q_start, 1, torch.int32, self.device)
-        _check("kv_len", kv_len, 1, torch.int32, self.device)
+        _check("page_table", page_table, 2, torch.int32, device)
+        _check("q_start", q_start, 1, torch.int32, device)
+        _check("kv_len", kv_len, 1, torch.int32, device)
         seqs, width = page_table.shape
         if seqs > self.max_seqs or q_start.shape[0] != seqs + 1 or kv_len.shape[0] != seqs:
             raise KernelBuildError(
                 f"{seqs} sequences in page_table, {q_start.shape[0] - 1} in q_start, "
                 f"{kv_len.shape[0]} in kv_len; at most {self.max_seqs}")
-        if (width > 1 and page_table.stride(1) != 1) or not q_start.is_contiguous() \
+        row, step = page_table.stride()
+        if (width > 1 and step != 1) or not q_start.is_contiguous() \
                 or not kv_len.is_contiguous():
             raise KernelBuildError("page_table rows, q_start and kv_len must be contiguous")
-        a.num_seqs, a.tokens, a.num_pages = seqs, rows, k_pages.shape[0]
-        a.table_width, a.table_stride = width, page_table.stride(0)
-        a.page_table, a.q_start, a.kv_len = (page_table.data_ptr(), q_start.data_ptr(),
-                                             kv_len.data_ptr())
-        _heads(a.k_pages, k_pages)
-        _heads(a.v_pages, v_pages)
+        at = _lib.GpoPagedArgs
+        _PAGED_SIZES.pack_into(a, at.num_seqs.offset, seqs, rows)
+        _PAGED_PAGES.pack_into(a, at.num_pages.offset, pages)
+        _PAGED_TABLE.pack_into(a, at.table_width.offset, width, row)
+        _PAGED_HEADS.pack_into(a, at.k_pages.offset, *_heads(k_pages), *_heads(v_pages))
+        _PAGED_PTRS.pack_into(a, at.page_table.offset, page_table.data_ptr(), q_start.data_ptr(),
+                              kv_len.data_ptr(), lse)
         return a
 
     def append(self, k, v, k_pages, v_pages, page_table, q_start, kv_len) -> None:
@@ -276,8 +307,7 @@ class PagedAttention:
                                        f"{self.heads_kv}, {self.head_dim})")
         k, v = _readable(k), _readable(v)
         a = self._fill(k.shape[0], k_pages, v_pages, page_table, q_start, kv_len)
-        _heads(a.k_new, k)
-        _heads(a.v_new, v)
+        _PAGED_HEADS.pack_into(a, _lib.GpoPagedArgs.k_new.offset, *_heads(k), *_heads(v))
         _launch("gpo_cache_append", a, self.device)
 
     def attend(self, q, k_pages, v_pages, page_table, q_start, kv_len, out=None,
@@ -292,18 +322,18 @@ class PagedAttention:
                                    f"{self.heads_q}, {self.head_dim})")
         q = _readable(q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         else:
             _check("out", out, 3, self.dtype, self.device)
-            if out.shape != q.shape or out.stride(2) != 1:
-                raise KernelBuildError(f"out must be like q {tuple(q.shape)}, rows contiguous")
+            if out.shape != q.shape or not _in_place(out):
+                raise KernelBuildError(f"out must have q's shape {tuple(q.shape)}, its rows "
+                                       "contiguous and 16-byte aligned")
         if lse is not None:
             _check("lse", lse, 2, torch.float32, self.device)
             if lse.shape != q.shape[:2] or not lse.is_contiguous():
                 raise KernelBuildError(f"lse must be a contiguous {tuple(q.shape[:2])} tensor")
-        a = self._fill(q.shape[0], k_pages, v_pages, page_table, q_start, kv_len)
-        _heads(a.q, q)
-        _heads(a.out, out)
-        a.lse = 0 if lse is None else lse.data_ptr()
+        a = self._fill(q.shape[0], k_pages, v_pages, page_table, q_start, kv_len,
+                       0 if lse is None else lse.data_ptr())
+        _PAGED_HEADS.pack_into(a, _lib.GpoPagedArgs.q.offset, *_heads(q), *_heads(out))
         _launch("gpo_paged_attention", a, self.device)
         return out

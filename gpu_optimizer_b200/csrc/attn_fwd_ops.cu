@@ -5,36 +5,61 @@
 // log-sum-exp of its scaled scores.  One pass over the visible K/V blocks
 // with the running maximum and sum of each row in registers.
 //
-// One CTA per SM works through tiles of 128 query rows (attn_ops.cuh: a
-// tile packs all query heads of a kv head, so K/V is read once per kv head):
-//   warp 0  TMA of Q and of the K ring
-//   warp 3  TMA of the V ring; clears V rows behind a sequence's last key
-//   warp 1  MMA issuer: S_j = Q K_j^T into TMEM buffer j % 3, two blocks
-//           ahead of O += P_j V_j (P overlays S as 16-bit pairs)
-//   warp 2  TMEM owner
-//   warps 4-7  softmax: thread = query row = TMEM lane
+// A unit of work is a span of TILES tiles of 128 query rows of one sequence
+// and kv head (attn_ops.cuh: a tile packs all query heads of the kv head,
+// so K/V is read once for all of them).  One persistent CTA per SM:
+//   warp 0     TMA of Q and of the K ring
+//   warp 3     TMA of the V ring; clears V rows behind a sequence's last key
+//   warp 1     MMA issuer; P overlays S in TMEM as 16-bit pairs
+//   warp 2     TMEM owner
+//   warps 4-7  softmax and epilogue of tile 0, thread = query row = TMEM
+//   warps 8-11 lane; of tile 1
+// TILES = 2 (more than 128 rows per sequence and kv head): both tiles share
+// every K/V block; the issuer alternates them, so that one tile's softmax
+// hides behind the other's MMAs.  TILES = 1 (single tokens, short chunks):
+// bound by the K/V bytes; three S buffers let S run two blocks ahead of PV.
+//
 // Only blocks with a visible key are loaded.  A page that ends inside a
 // block is loaded as boxes of its own rows; boxes without a key are asked
 // for outside the tensor, which TMA fills with zeros.
+//
+// Whole units (many of them) are dealt out in rounds, the longest rows first
+// and every other round backwards.  Few units (STREAM, paged only) are cut: all units' blocks form one
+// line, and every CTA takes an equal stretch of it, whatever the lengths of
+// the sequences, which only the device knows.  A unit that lies in one
+// stretch is finished by its CTA; of one that is cut, every CTA writes its
+// part (O unnormalised, maximum, sum) to the workspace and the CTA that
+// arrives last joins the parts in their order.
 #include <algorithm>
 
 #include "attn_ops.cuh"
 
 namespace gpo {
 
-constexpr int kFwdStages = 3;   // K slots and V slots
-constexpr int kFwdSBufs = 3;    // S/P buffers in TMEM
-constexpr int kFwdThreads = 256;
-constexpr float kFwdRescale = 8.0f;  // see the softmax
+constexpr int kFwdMaxStages = 3;       // slots of the K ring and of the V ring
+constexpr int kFwdSBufs = 3;           // S/P buffers (TILES = 1)
+constexpr float kFwdRescale = 8.0f;    // see the softmax
+constexpr int kFwdMaxCtas = 160;       // CTAs that a workspace has room for
+constexpr int kFwdStreamPairs = 1024;  // most (sequence, span) pairs of a cut launch
+// Registers of TILES = 2: 384 threads launch at 168; 128 * 88 + 256 * 208 is
+// the same total (a softmax thread holds a row of 128 scores).
+constexpr int kFwdLowRegs = 88, kFwdHighRegs = 208;
+static_assert(128 * kFwdLowRegs + 256 * kFwdHighRegs <= 168 * 384,
+              "register split exceeds the launch's registers");
 
 struct FwdShared {
   uint64_t q_full, q_empty;
-  uint64_t k_full[kFwdStages], k_empty[kFwdStages];
-  uint64_t v_full[kFwdStages], v_empty[kFwdStages];
-  uint64_t v_clean[kFwdStages];  // the slot's block has been cleared behind the last key
-  uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], pv_done[kFwdSBufs];
-  uint64_t o_full, o_free;
+  uint64_t k_full[kFwdMaxStages], k_empty[kFwdMaxStages];
+  uint64_t v_full[kFwdMaxStages], v_empty[kFwdMaxStages];
+  uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared behind the last key
+  uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], p_half[2], pv_done[kFwdSBufs];
+  uint64_t o_full[2], o_free[2];
   uint64_t drain;
+  // cut launches: where this CTA's stretch begins
+  int64_t line_pos, line_end, line_len;
+  int64_t warp_sum[8];
+  int line_pair, line_head, line_off;
+  int last[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -45,7 +70,13 @@ struct FwdArgs {
   float* lse;  // (batch, q_len, heads) or (tokens, heads); may be null
   int64_t o_batch, o_token, o_head;
   float scale_log2;
+  int spans;     // units of a sequence and kv head (of the longest sequence)
   int items;
+  int stages;
+  // cut launches
+  unsigned int* arrived;  // per unit and tile, 0 between launches
+  float* part;            // [CTA][2] parts of part_rows rows: D floats each, then (m, l)
+  int part_rows;
   unsigned int* err;
 };
 
@@ -60,303 +91,567 @@ struct RingPos2 {
   }
 };
 
-// One work item: a tile of query rows of one sequence and kv head.
-struct FwdItem {
-  int b, h, t0, t1;
+// A stretch of a unit: blocks [i0, i1) of the n that its span sees.
+struct FwdSeg {
+  int b, h, t0, t1;  // tokens [t0, t1) of the span
   AttnSeq seq;
   AttnBlocks blk;
+  int i0, i1;
+  int64_t line0;  // cut launches: position of the unit's first block
+  int unit;
+  bool whole;
 };
 
-template <bool PAGED>
-__device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item) {
-  const AttnGeom& g = a.geom;
-  FwdItem it;
-  it.h = item % g.heads_kv;
-  const int r = item / g.heads_kv;
-  it.b = r % g.batch;
-  const int tile = g.tiles - 1 - r / g.batch;  // the longest rows first
-  it.seq = attn_seq<PAGED>(g, it.b, a.err);
-  it.t0 = tile * g.tpt;
-  it.t1 = min(it.t0 + g.tpt, it.seq.q_len);
-  it.blk = attn_blocks(g, it.seq, it.t0, it.t1);
-  return it;
+// The CTA's stretches in order; every role walks them by itself.
+template <bool PAGED, bool STREAM, int TILES>
+struct FwdWalk {
+  const FwdArgs& a;
+  FwdSeg s;
+  int item, turn;     // whole units: first item of the CTA's turn
+  int64_t pos, end;   // cut: positions in the line of blocks
+  int pair, head, off, n, known;
+
+  __device__ __forceinline__ FwdWalk(const FwdArgs& args, const FwdShared& sh) : a(args) {
+    item = 0;
+    turn = 0;
+    if constexpr (STREAM) {
+      pos = sh.line_pos;
+      end = sh.line_end;
+      pair = sh.line_pair;
+      head = sh.line_head;
+      off = sh.line_off;
+      known = -1;
+      n = 0;
+    }
+  }
+
+  __device__ __forceinline__ void place(int r) {
+    const AttnGeom& g = a.geom;
+    s.b = r % g.batch;
+    s.seq = attn_seq<PAGED>(g, s.b, a.err);
+    s.t0 = (a.spans - 1 - r / g.batch) * TILES * g.tpt;  // the longest rows first
+    s.t1 = min(s.t0 + TILES * g.tpt, s.seq.q_len);
+    s.blk = attn_blocks(g, s.seq, s.t0, s.t1);
+  }
+
+  // The next stretch with a query (its rows may see no key: i0 == i1).
+  __device__ __forceinline__ bool next() {
+    const AttnGeom& g = a.geom;
+    if constexpr (!STREAM) {
+      // The longest units come first, and every other round runs backwards:
+      // a CTA that had the longest of a round takes the shortest of the next.
+      while (item < a.items) {
+        const int mine = item + static_cast<int>((turn & 1) ? gridDim.x - 1 - blockIdx.x
+                                                            : blockIdx.x);
+        item += gridDim.x;
+        ++turn;
+        if (mine >= a.items) continue;
+        s.h = mine % g.heads_kv;
+        place(mine / g.heads_kv);
+        if (s.t0 >= s.t1) continue;
+        s.i0 = 0;
+        s.i1 = s.blk.n;
+        s.whole = true;
+        return true;
+      }
+      return false;
+    } else {
+      if (pos >= end) return false;
+      while (known != pair) {
+        place(pair);
+        known = pair;
+        n = s.t0 < s.t1 ? max(1, s.blk.n) : 0;  // rows without a key: one empty block
+        if (n == 0) ++pair;
+      }
+      s.h = head;
+      s.unit = pair * g.heads_kv + head;
+      s.line0 = pos - off;
+      s.i0 = off;
+      s.i1 = static_cast<int>(min(static_cast<int64_t>(n), off + (end - pos)));
+      s.whole = s.i0 == 0 && s.i1 == n;
+      pos += s.i1 - s.i0;
+      off = s.i1;
+      if (off == n) {
+        off = 0;
+        if (++head == g.heads_kv) {
+          head = 0;
+          ++pair;
+        }
+      }
+      if (s.blk.n == 0) s.i1 = s.i0;
+      return true;
+    }
+  }
+};
+
+// Tile t of a stretch: its tokens and which of the span's blocks it sees.
+struct FwdTile {
+  int t0, t1, first, last, sinks;
+  __device__ __forceinline__ bool sees(int block) const {
+    return block <= last && (block >= first || block < sinks);
+  }
+};
+
+__device__ __forceinline__ FwdTile fwd_tile(const AttnGeom& g, const FwdSeg& s, int t) {
+  FwdTile f;
+  f.t0 = s.t0 + t * g.tpt;
+  f.t1 = min(f.t0 + g.tpt, s.seq.q_len);
+  const AttnBlocks b = attn_blocks(g, s.seq, f.t0, f.t1);
+  f.first = b.first;
+  f.sinks = b.sink_blocks;
+  f.last = b.n > 0 ? b.first + b.n - b.sink_blocks - 1 : -1;
+  return f;
 }
 
-template <typename T, int FMT, int D, bool PAGED>
-__global__ void __launch_bounds__(kFwdThreads, 1)
-    attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q,
-                    const __grid_constant__ CUtensorMap tma_k,
-                    const __grid_constant__ CUtensorMap tma_v,
-                    const __grid_constant__ FwdArgs args) {
-  constexpr int BN = kOpsBN;
-  constexpr int SW = 128;               // swizzle atom: 64 dims of a row
-  constexpr int ATOMS = D / 64;
-  constexpr uint32_t Q_BYTES = 128u * D * 2;
-  constexpr uint32_t KV_BYTES = static_cast<uint32_t>(BN) * D * 2;
-  constexpr int NB = kFwdSBufs, LAG = NB - 1;
+// Cut launches: the blocks of every (sequence, span) pair are counted, and
+// the pair where this CTA's stretch begins is found by a prefix sum.
+template <bool PAGED, int TILES>
+__device__ __forceinline__ void fwd_stretch(const FwdArgs& a, FwdShared& sh) {
+  const AttnGeom& g = a.geom;
+  const int pairs = a.spans * g.batch;
+  const int per = (pairs + 255) / 256;
+  const int tid = threadIdx.x, lane = tid & 31;
+  FwdWalk<PAGED, false, TILES> w(a, sh);
+  int cnt[kFwdStreamPairs / 256];
+  int64_t mine = 0;
+  if (tid < 256) {
+#pragma unroll
+    for (int i = 0; i < kFwdStreamPairs / 256; ++i) {
+      cnt[i] = 0;
+      const int r = tid * per + i;
+      if (i < per && r < pairs) {
+        w.place(r);
+        cnt[i] = w.s.t0 < w.s.t1 ? max(1, w.s.blk.n) : 0;
+        mine += cnt[i];
+      }
+    }
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (tid < 256 && lane == 31) sh.warp_sum[tid >> 5] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i < (tid >> 5)) before += sh.warp_sum[i];
+    total += sh.warp_sum[i];
+  }
+  total *= g.heads_kv;
+  const int64_t len = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t p0 = min(total, len * blockIdx.x), p1 = min(total, p0 + len);
+  if (tid == 0) {
+    sh.line_pos = p0;
+    sh.line_end = p1;
+    sh.line_len = len;
+  }
+  if (tid < 256) {
+#pragma unroll
+    for (int i = 0; i < kFwdStreamPairs / 256; ++i) {
+      const int64_t b0 = before * g.heads_kv, b1 = b0 + static_cast<int64_t>(cnt[i]) * g.heads_kv;
+      if (p0 < p1 && p0 >= b0 && p0 < b1) {
+        sh.line_pair = tid * per + i;
+        sh.line_head = static_cast<int>((p0 - b0) / cnt[i]);
+        sh.line_off = static_cast<int>((p0 - b0) % cnt[i]);
+      }
+      before += cnt[i];
+    }
+  }
+}
+
+// Floats of a part: rows of O, then (m, l) of each row, on 16 bytes.
+__host__ __device__ constexpr int64_t fwd_part_floats(int64_t rows, int d) {
+  return rows * d + ((2 * rows + 3) & ~static_cast<int64_t>(3));
+}
+
+template <int N>
+__device__ __forceinline__ void fwd_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fwd_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ void fwd_barrier(int id) {
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+}
+
+template <int D>
+struct FwdGeom {
+  static constexpr int SW = 128;  // swizzle atom: 64 dims of a row
+  static constexpr int ATOMS = D / 64;
+  static constexpr uint32_t Q_BYTES = 128u * D * 2;
+  static constexpr uint32_t KV_BYTES = static_cast<uint32_t>(kOpsBN) * D * 2;
+};
+
+// ---------------------------------------------------------------- producer
+// K ring and Q (is_k), or V ring.  The whole warp runs the loop: each lane
+// loads one box of a block.
+template <int D, bool PAGED, bool STREAM, int TILES>
+__device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
+                                             const CUtensorMap* tma_q, const CUtensorMap* map,
+                                             uint32_t q_smem, uint32_t ring, bool is_k, int lane) {
+  using G = FwdGeom<D>;
+  const AttnGeom& g = args.geom;
+  uint64_t* full = is_k ? sh.k_full : sh.v_full;
+  uint64_t* empty = is_k ? sh.k_empty : sh.v_empty;
+  volatile int* abort_flag = &sh.abort;
+  const int boxes = PAGED ? kOpsBN / g.box_rows : 1;
+  bool ok = true;
+  int issued = 0, q_loads = 0;
+  RingPos2 pos;
+  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
+  while (ok && w.next()) {
+    const FwdSeg& s = w.s;
+    if (s.i0 == s.i1) continue;
+    if (is_k) {
+      // Q of the previous stretch is free once its last S MMA is done
+      ok = q_loads == 0 || mbar_wait(smem_u32(&sh.q_empty), (q_loads - 1) & 1u, abort_flag,
+                                     args.err, kErrWaitProducer);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(smem_u32(&sh.q_full),
+                              static_cast<uint32_t>(TILES * g.tpt * g.g) * D * 2);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int c = 0; c < G::ATOMS; ++c)
+            tma_load_5d(q_smem + t * G::Q_BYTES + c * 128 * G::SW, tma_q, smem_u32(&sh.q_full),
+                        c * 64, 0, s.h, s.seq.row0 + s.t0 + t * g.tpt, PAGED ? 0 : s.b);
+      }
+      ++q_loads;
+    }
+    for (int i = s.i0; i < s.i1; ++i) {
+      const int key0 = s.blk.at(i) * kOpsBN;
+      int page = s.b, row = key0;
+      if constexpr (PAGED) {
+        const int key = key0 + lane * g.box_rows;
+        page = g.num_pages;  // outside the tensor: zeros
+        if (lane < boxes && key < s.seq.kv_len)
+          page = __ldg(g.table + s.b * g.table_stride + key / g.page_size);
+        row = key % g.page_size;
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[pos.slot]), pos.parity ^ 1u,
+                                             abort_flag, args.err, kErrWaitProducer));
+      if (!ok) break;
+      const uint32_t bar = smem_u32(&full[pos.slot]);
+      const uint32_t slot = ring + pos.slot * G::KV_BYTES;
+      if (lane == 0) mbar_arrive_expect_tx(bar, G::KV_BYTES);
+      __syncwarp();
+      if (lane < boxes) {
+        const uint32_t dst = slot + static_cast<uint32_t>(PAGED ? lane * g.box_rows : 0) * G::SW;
+#pragma unroll
+        for (int c = 0; c < G::ATOMS; ++c)
+          tma_load_4d(dst + c * kOpsBN * G::SW, map, bar, c * 64, s.h, row, page);
+      }
+      ++issued;
+      if (PAGED && !is_k && key0 + kOpsBN > s.seq.kv_len) {
+        // Slots behind a sequence's last key hold anything; P is 0 there,
+        // but 0 * NaN is not: their V rows are cleared in shared memory
+        // before the MMA reads the block (always a unit's last one).
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(bar, pos.parity, abort_flag, args.err, kErrWaitProducer));
+        if (!ok) break;
+        for (int r = s.seq.kv_len - key0; r < kOpsBN; ++r)
+          if (lane < G::ATOMS * 8)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             slot + (lane / 8) * kOpsBN * G::SW + r * G::SW + (lane % 8) * 16),
+                         "r"(0)
+                         : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[pos.slot]));
+      }
+      pos.step(args.stages);
+    }
+  }
+  if (!ok && lane == 0) {
+    // let the copies in flight land before the CTA can exit
+    if (q_loads > 0) mbar_wait_drain(smem_u32(&sh.q_full), (q_loads - 1) & 1u, args.err);
+    for (int j = max(0, issued - args.stages); j < issued; ++j)
+      mbar_wait_drain(smem_u32(&full[j % args.stages]), (j / args.stages) & 1u, args.err);
+  }
+}
+
+// -------------------------------------------------------------- MMA issuer
+template <int FMT, int D, bool PAGED, bool STREAM, int TILES>
+__device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint32_t tmem,
+                                        uint32_t q_smem, uint32_t k_smem, uint32_t v_smem) {
+  using G = FwdGeom<D>;
+  constexpr int BN = kOpsBN, SW = G::SW;
   constexpr uint32_t IDESC_S = make_idesc(FMT, 128, BN, false, false);
   constexpr uint32_t IDESC_O = make_idesc(FMT, 128, D, false, true);
-  static_assert(D + NB * BN <= 512, "TMEM holds 512 columns");
-
-  __shared__ FwdShared sh;
-  extern __shared__ uint8_t dyn_smem[];
-  const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
-  const uint32_t q_smem = base;
-  const uint32_t k_smem = q_smem + Q_BYTES;
-  const uint32_t v_smem = k_smem + kFwdStages * KV_BYTES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t S_COL = TILES * D;  // S/P buffers behind the O tiles
+  constexpr uint64_t HI = smem_desc_hi(8 * SW, SW);
   const AttnGeom& g = args.geom;
   unsigned int* err = args.err;
-
-  if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&sh.q_full), 1);
-    mbar_init(smem_u32(&sh.q_empty), 1);
-    for (int s = 0; s < kFwdStages; ++s) {
-      mbar_init(smem_u32(&sh.k_full[s]), 1);
-      mbar_init(smem_u32(&sh.k_empty[s]), 1);
-      mbar_init(smem_u32(&sh.v_full[s]), 1);
-      mbar_init(smem_u32(&sh.v_empty[s]), 1);
-      mbar_init(smem_u32(&sh.v_clean[s]), 1);
-    }
-    for (int b = 0; b < NB; ++b) {
-      mbar_init(smem_u32(&sh.s_full[b]), 1);
-      mbar_init(smem_u32(&sh.p_full[b]), 4);
-      mbar_init(smem_u32(&sh.pv_done[b]), 1);
-    }
-    mbar_init(smem_u32(&sh.o_full), 1);
-    mbar_init(smem_u32(&sh.o_free), 4);
-    mbar_init(smem_u32(&sh.drain), 1);
-    sh.abort = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&tma_q);
-    tma_prefetch_desc(&tma_k);
-    tma_prefetch_desc(&tma_v);
-  }
-  if (warp == 2) {
-    tmem_alloc(smem_u32(&sh.tmem_base), 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem_base;
   volatile int* abort_flag = &sh.abort;
-
-  if (warp == 0 || warp == 3) {
-    // ------------------------------------------- producers (K: 0, V: 3)
-    // The whole warp runs the loop: each lane loads one box of a block.
-    const bool is_k = warp == 0;
-    const CUtensorMap* map = is_k ? &tma_k : &tma_v;
-    const uint32_t ring = is_k ? k_smem : v_smem;
-    uint64_t* full = is_k ? sh.k_full : sh.v_full;
-    uint64_t* empty = is_k ? sh.k_empty : sh.v_empty;
-    const int boxes = PAGED ? BN / g.box_rows : 1;
-    bool ok = true;
-    int issued = 0, q_loads = 0;
-    RingPos2 pos;
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const FwdItem it = fwd_item<PAGED>(args, item);
-      if (it.blk.n == 0) continue;
-      if (is_k) {
-        // Q of the previous item is free once its last S MMA is done
-        ok = q_loads == 0 || mbar_wait(smem_u32(&sh.q_empty), (q_loads - 1) & 1u, abort_flag,
-                                       err, kErrWaitProducer);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(smem_u32(&sh.q_full),
-                                static_cast<uint32_t>(g.tpt * g.g) * D * 2);
+  const int stages = args.stages;
+  // Between two MMA groups this thread does as little as it can: descriptor
+  // halves advance by constants, waits test the phase without blocking first.
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    const uint32_t b = smem_u32(bar);
+    return mbar_test_wait(b, parity) || mbar_wait(b, parity, abort_flag, err, kErrWaitMma);
+  };
+  const uint32_t q_lo = smem_desc_lo(q_smem, 16);
+  const uint32_t k_lo = smem_desc_lo(k_smem, 16);
+  const uint32_t v_lo = smem_desc_lo(v_smem, BN * SW);
+  auto s_mma = [&](int t, int buf, int k_slot) {
+    const uint32_t qd = q_lo + t * (G::Q_BYTES >> 4), kd = k_lo + k_slot * (G::KV_BYTES >> 4);
 #pragma unroll
-          for (int c = 0; c < ATOMS; ++c)
-            tma_load_5d(q_smem + c * 128 * SW, &tma_q, smem_u32(&sh.q_full), c * 64, 0, it.h,
-                        it.seq.row0 + it.t0, PAGED ? 0 : it.b);
-        }
-        ++q_loads;
-      }
-      for (int i = 0; i < it.blk.n; ++i) {
-        const int key0 = it.blk.at(i) * BN;
-        int page = it.b, row = key0;
-        if constexpr (PAGED) {
-          const int key = key0 + lane * g.box_rows;
-          page = g.num_pages;  // outside the tensor: zeros
-          if (lane < boxes && key < it.seq.kv_len)
-            page = __ldg(g.table + it.b * g.table_stride + key / g.page_size);
-          row = key % g.page_size;
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[pos.slot]), pos.parity ^ 1u,
-                                               abort_flag, err, kErrWaitProducer));
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&full[pos.slot]);
-        if (lane == 0) mbar_arrive_expect_tx(bar, KV_BYTES);
-        __syncwarp();
-        if (lane < boxes) {
-          const uint32_t dst = ring + pos.slot * KV_BYTES +
-                               static_cast<uint32_t>(PAGED ? lane * g.box_rows : 0) * SW;
-#pragma unroll
-          for (int c = 0; c < ATOMS; ++c)
-            tma_load_4d(dst + c * BN * SW, map, bar, c * 64, it.h, row, page);
-        }
-        ++issued;
-        if (PAGED && !is_k && key0 + BN > it.seq.kv_len) {
-          // Slots behind a sequence's last key hold anything; P is 0 there,
-          // but 0 * NaN is not: their V rows are cleared in shared memory
-          // before the MMA reads the block (always an item's last one).
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(bar, pos.parity, abort_flag, err, kErrWaitProducer));
-          if (!ok) break;
-          for (int r = it.seq.kv_len - key0; r < BN; ++r)
-            if (lane < ATOMS * 8)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                               v_smem + pos.slot * KV_BYTES + (lane / 8) * BN * SW + r * SW +
-                               (lane % 8) * 16),
-                           "r"(0)
-                           : "memory");
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[pos.slot]));
-        }
-        pos.step(kFwdStages);
-      }
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = ((kk / 4) * 128 * SW + (kk % 4) * 32) >> 4;
+      mma_f16_ss(tmem + S_COL + buf * BN, HI | (qd + off), HI | (kd + off), IDESC_S,
+                 kk > 0 ? 1u : 0u);
     }
-    if (!ok && lane == 0) {
-      // let the copies in flight land before the CTA can exit
-      if (q_loads > 0) mbar_wait_drain(smem_u32(&sh.q_full), (q_loads - 1) & 1u, err);
-      for (int j = max(0, issued - kFwdStages); j < issued; ++j)
-        mbar_wait_drain(smem_u32(&full[j % kFwdStages]), (j / kFwdStages) & 1u, err);
+    mma_commit(smem_u32(&sh.s_full[buf]));
+  };
+  auto pv_part = [&](int t, int buf, int v_slot, int k0, int k1, bool first) {
+    const uint32_t vd = v_lo + v_slot * (G::KV_BYTES >> 4);
+    for (int kk = k0; kk < k1; ++kk)
+      mma_f16_ts(tmem + t * D, tmem + S_COL + buf * BN + kk * 8,
+                 HI | (vd + ((kk * 16 * SW) >> 4)), IDESC_O, (first && kk == 0) ? 0u : 1u);
+  };
+  bool ok = true;
+  RingPos2 kpos, vpos;
+  uint32_t cleaned = 0;  // bit s: parity of slot s's next v_clean phase
+  auto wait_v = [&](const FwdSeg& s, int i) {
+    if (!wait(&sh.v_full[vpos.slot], vpos.parity)) return false;
+    if (PAGED && (s.blk.at(i) + 1) * BN > s.seq.kv_len) {
+      if (!wait(&sh.v_clean[vpos.slot], (cleaned >> vpos.slot) & 1u)) return false;
+      cleaned ^= 1u << vpos.slot;
     }
-  } else if (warp == 1 && lane == 0) {
-    // ------------------------------------------------------- MMA issuer
-    constexpr uint64_t HI = smem_desc_hi(8 * SW, SW);
-    const uint32_t q_lo = smem_desc_lo(q_smem, 16);
-    const uint32_t k_lo = smem_desc_lo(k_smem, 16);
-    const uint32_t v_lo = smem_desc_lo(v_smem, BN * SW);
-    bool ok = true;
-    RingPos2 kpos, vpos, spos, ppos;
-    uint32_t items_done = 0;
-    uint32_t cleaned = 0;  // bit s: parity of slot s's next v_clean phase
-    auto wait = [&](const uint64_t* bar, uint32_t parity) {
-      return mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitMma);
-    };
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const FwdItem it = fwd_item<PAGED>(args, item);
-      const int n = it.blk.n;
+    return true;
+  };
+  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
+  uint32_t segs = 0;
+  if constexpr (TILES == 1) {
+    constexpr int NB = kFwdSBufs, LAG = NB - 1;
+    RingPos2 spos, ppos;
+    while (ok && w.next()) {
+      const FwdSeg& s = w.s;
+      const int n = s.i1 - s.i0;
       if (n == 0) continue;
-      ok = wait(&sh.q_full, items_done & 1u);
+      ok = wait(&sh.q_full, segs & 1u);
       for (int i = 0; i < n + LAG && ok; ++i) {
         if (i < n) {
           // S buffer i % NB last held P of block i - NB, whose PV MMA was
           // issued before; MMAs of one thread execute in issue order
           ok = wait(&sh.k_full[kpos.slot], kpos.parity);
           if (!ok) break;
-          tc_fence_after();
-          const uint32_t s_tmem = tmem + D + spos.slot * BN;
-          const uint32_t kd = k_lo + kpos.slot * (KV_BYTES >> 4);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk / 4) * 128 * SW + (kk % 4) * 32) >> 4;
-            mma_f16_ss(s_tmem, HI | (q_lo + off), HI | (kd + off), IDESC_S, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(smem_u32(&sh.s_full[spos.slot]));
+          s_mma(0, spos.slot, kpos.slot);
           mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
           if (i == n - 1) mma_commit(smem_u32(&sh.q_empty));
-          kpos.step(kFwdStages);
+          kpos.step(stages);
           spos.step(NB);
         }
         const int j = i - LAG;
-        if (j >= 0 && j < n) {
-          ok = wait(&sh.v_full[vpos.slot], vpos.parity) &&
-               wait(&sh.p_full[ppos.slot], ppos.parity);
-          // the first PV overwrites O: the last item's epilogue has read it
-          if (ok && j == 0 && items_done > 0) ok = wait(&sh.o_free, (items_done - 1) & 1u);
-          if (PAGED && ok && (it.blk.at(j) + 1) * BN > it.seq.kv_len) {
-            ok = wait(&sh.v_clean[vpos.slot], (cleaned >> vpos.slot) & 1u);
-            cleaned ^= 1u << vpos.slot;
-          }
+        if (j >= 0) {
+          ok = wait_v(s, s.i0 + j) && wait(&sh.p_full[ppos.slot], ppos.parity);
+          // the first PV overwrites O: the last epilogue has read it
+          if (ok && j == 0 && segs > 0) ok = wait(&sh.o_free[0], (segs - 1) & 1u);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t p_tmem = tmem + D + ppos.slot * BN;
-          const uint32_t vd = v_lo + vpos.slot * (KV_BYTES >> 4);
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            mma_f16_ts(tmem, p_tmem + kk * 8, HI | (vd + ((kk * 16 * SW) >> 4)), IDESC_O,
-                       (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; kk += 4)
+            pv_part(0, ppos.slot, vpos.slot, kk, kk + 4, j == 0);
           mma_commit(smem_u32(&sh.pv_done[ppos.slot]));
           mma_commit(smem_u32(&sh.v_empty[vpos.slot]));
-          if (j == n - 1) mma_commit(smem_u32(&sh.o_full));
-          vpos.step(kFwdStages);
+          if (j == n - 1) mma_commit(smem_u32(&sh.o_full[0]));
+          vpos.step(stages);
           ppos.step(NB);
         }
       }
-      ++items_done;
+      ++segs;
     }
-    if (!ok) {
-      mma_commit(smem_u32(&sh.drain));
-      mbar_wait_drain(smem_u32(&sh.drain), 0, err);
-    }
-  } else if (warp >= 4) {
-    // ------------------------------------------------ softmax, epilogue
-    const int q = warp & 3;
-    const int row = q * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t o_tmem = tmem + lane_addr;
-    const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
-    const int row_token = row / g.g, row_head = row % g.g;
-    bool ok = true;
-    RingPos2 spos, last_pv;
-    uint32_t items_done = 0;
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const FwdItem it = fwd_item<PAGED>(args, item);
-      if (it.t0 >= it.t1) continue;
-      const int token = it.t0 + row_token;
-      const bool live = row_token < g.tpt && token < it.t1;
-      const int p = token + it.seq.off;
-      float m_used = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.blk.n; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.s_full[spos.slot]), spos.parity,
-                                               abort_flag, err, kErrWaitSoftmax));
+  } else {
+    uint32_t blocks[2] = {0u, 0u};  // blocks of each tile so far: phases of its P
+    uint32_t outs[2] = {0u, 0u};    // stretches in which the tile had a block
+    while (ok && w.next()) {
+      const FwdSeg& s = w.s;
+      if (s.i0 == s.i1) continue;
+      const FwdTile tile[2] = {fwd_tile(g, s, 0), fwd_tile(g, s, 1)};
+      auto sees = [&](int t, int i) { return tile[t].sees(s.blk.at(i)); };
+      bool begun[2] = {false, false};
+      ok = wait(&sh.q_full, segs & 1u) && wait(&sh.k_full[kpos.slot], kpos.parity);
+      if (!ok) break;
+      // S_t of a stretch's first block overwrites the P that the last PV_t of
+      // the stretch before read: it was issued before, MMAs run in order
+      bool now[2], then[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        now[t] = sees(t, s.i0);
+        if (now[t]) s_mma(t, t, kpos.slot);
+      }
+      mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
+      kpos.step(stages);
+      if (s.i1 - s.i0 == 1) mma_commit(smem_u32(&sh.q_empty));
+      for (int i = s.i0; i < s.i1; ++i) {
+        const bool more = i + 1 < s.i1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) then[t] = more && sees(t, i + 1);
+        ok = wait_v(s, i);
         if (!ok) break;
-        if (q * 32 >= (it.t1 - it.t0) * g.g) {
-          // no row of this warp holds a query (short chunks, single
-          // tokens): whatever its P rows hold reaches only its own O rows
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[spos.slot]));
-          spos.step(NB);
-          continue;
+        bool k_ready = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (now[t]) {
+            // a tile's first PV overwrites O_t: the last epilogue has read it
+            if (!begun[t] && outs[t] > 0) ok = wait(&sh.o_free[t], (outs[t] - 1) & 1u);
+            if (!ok) break;
+            // keys [0, 64) as soon as their P is stored, then the rest
+            const uint32_t par = blocks[t] & 1u;
+            const bool all = mbar_test_wait(smem_u32(&sh.p_full[t]), par);
+            if (!all) {
+              ok = wait(&sh.p_half[t], par);
+              if (!ok) break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < BN / 32; ++kk)
+              pv_part(t, t, vpos.slot, kk, kk + 1, !begun[t]);
+            if (!all) {
+              ok = wait(&sh.p_full[t], par);
+              if (!ok) break;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int kk = BN / 32; kk < BN / 16; ++kk)
+              pv_part(t, t, vpos.slot, kk, kk + 1, false);
+            begun[t] = true;
+            ++blocks[t];
+            if (!then[t]) {
+              // the tile's last block, unless it skips some (a gap between
+              // its sinks and its window that the other tile sees)
+              bool end = true;
+              for (int x = i + 2; x < s.i1 && end; ++x) end = !sees(t, x);
+              if (end) {
+                mma_commit(smem_u32(&sh.o_full[t]));
+                ++outs[t];
+              }
+            }
+          }
+          if (then[t]) {
+            if (!k_ready) {
+              ok = wait(&sh.k_full[kpos.slot], kpos.parity);
+              if (!ok) break;
+              k_ready = true;
+            }
+            s_mma(t, t, kpos.slot);
+          }
         }
+        if (ok && more && !k_ready) ok = wait(&sh.k_full[kpos.slot], kpos.parity);
+        if (!ok) break;
+        if (more) {
+          mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
+          if (i + 2 == s.i1) mma_commit(smem_u32(&sh.q_empty));
+          kpos.step(stages);
+        }
+        mma_commit(smem_u32(&sh.v_empty[vpos.slot]));
+        vpos.step(stages);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) now[t] = then[t];
+      }
+      ++segs;
+    }
+  }
+  if (!ok) {
+    mma_commit(smem_u32(&sh.drain));
+    mbar_wait_drain(smem_u32(&sh.drain), 0, err);
+  }
+}
+
+// ---------------------------------------------------- softmax and epilogue
+template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
+__device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, float2* join_ml,
+                                            uint32_t tmem, int warp, int lane) {
+  constexpr int BN = kOpsBN;
+  constexpr uint32_t S_COL = TILES * D;
+  const AttnGeom& g = args.geom;
+  unsigned int* err = args.err;
+  volatile int* abort_flag = &sh.abort;
+  const int t = TILES == 1 ? 0 : (warp - 4) >> 2;
+  const int q = warp & 3;
+  const int row = q * 32 + lane;
+  const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+  const uint32_t o_tmem = tmem + lane_addr + t * D;
+  const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
+  const int row_token = row / g.g, row_head = row % g.g;
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu,
+                      mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitSoftmax));
+  };
+  bool ok = true;
+  RingPos2 spos, last_pv;     // TILES = 1: S buffers
+  uint32_t blocks = 0, outs = 0;
+  if (TILES == 2) spos.slot = t;
+  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
+  while (ok && w.next()) {
+    const FwdSeg& s = w.s;
+    const FwdTile tile = fwd_tile(g, s, t);
+    if (tile.t0 >= tile.t1) continue;
+    const int token = tile.t0 + row_token;
+    const bool live = row_token < g.tpt && token < tile.t1;
+    const bool idle = q * 32 >= (tile.t1 - tile.t0) * g.g;  // no query in this warp
+    const int p = token + s.seq.off;
+    float m_used = -INFINITY, l = 0.f;
+    int seen = 0;
+    for (int i = s.i0; i < s.i1; ++i) {
+      if (TILES == 2 && !tile.sees(s.blk.at(i))) continue;
+      if (TILES == 2) spos.parity = blocks & 1u;
+      ok = wait(&sh.s_full[spos.slot], spos.parity);
+      if (!ok) break;
+      if (idle) {
+        // whatever the P rows of this warp hold reaches only its O rows
+        __syncwarp();
+        if (lane == 0) {
+          if (TILES == 2) mbar_arrive(smem_u32(&sh.p_half[t]));
+          mbar_arrive(smem_u32(&sh.p_full[spos.slot]));
+        }
+      } else {
         tc_fence_after();
-        const uint32_t sp = tmem + lane_addr + D + spos.slot * BN;
+        const uint32_t sp = tmem + lane_addr + S_COL + spos.slot * BN;
         uint32_t sv[BN];
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c)
           tmem_ld32(sp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
         tmem_wait_ld();
-        auto f = [&](int i) { return __uint_as_float(sv[i]); };
-        const int key0 = it.blk.at(j) * BN;
-        if (block_is_masked(g, it.seq, it.t0, it.t1, key0)) {
+        auto f = [&](int e) { return __uint_as_float(sv[e]); };
+        const int key0 = s.blk.at(i) * BN;
+        if (block_is_masked(g, s.seq, tile.t0, tile.t1, key0)) {
           const RowMask rm = row_mask(g, p, key0);
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (!rm.sees(i)) sv[i] = __float_as_uint(-INFINITY);
+          for (int c = 0; c < BN / 32; ++c) {
+            const uint32_t see = rm.word(c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              sv[c * 32 + e] = (see & (1u << e)) ? sv[c * 32 + e] : __float_as_uint(-INFINITY);
+          }
         }
         float mx[4] = {f(0), f(1), f(2), f(3)};
 #pragma unroll
-        for (int i = 4; i + 1 < BN; i += 2)
-          mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], f(i), f(i + 1));
+        for (int e = 4; e + 1 < BN; e += 2)
+          mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], f(e), f(e + 1));
         const float mb = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * args.scale_log2;
         // The maximum that P is taken against moves only when a block's
         // exceeds it by 2^8 (or there is none yet): P <= 256 is as exact in
         // 16 bits as P <= 1, and O is rescaled in TMEM that rarely.
-        if (j == 0) {
+        if (seen == 0) {
           m_used = mb;
         } else {
           const bool need = mb > m_used + kFwdRescale;
           if (__any_sync(0xffffffffu, need)) {
-            // O holds the PV of every earlier block once the last is done
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.pv_done[last_pv.slot]),
-                                                   last_pv.parity, abort_flag, err,
-                                                   kErrWaitSoftmax));
-            if (!ok) break;
-            tc_fence_after();
+            if (TILES == 1) {
+              // O holds the PV of every earlier block once the last is done
+              // (TILES = 2: S_t is issued behind the tile's last PV)
+              ok = wait(&sh.pv_done[last_pv.slot], last_pv.parity);
+              if (!ok) break;
+              tc_fence_after();
+            }
             const float m_new = need ? mb : m_used;
             const float alpha = need ? ex2_approx(m_used - m_new) : 1.f;
 #pragma unroll 1
@@ -365,7 +660,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
               tmem_ld16(o_tmem + c * 16, r);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+              for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
               tmem_st16(o_tmem + c * 16, r);
             }
             tmem_wait_st();
@@ -378,6 +673,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const float2 shift2 = make_float2(neg_m, neg_m);
         float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                         make_float2(0.f, 0.f)};
+        auto release = [&](uint64_t* bar) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(bar));
+        };
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t pk[16];
@@ -391,59 +692,250 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             pk[g2] = FMT == 1 ? pack_bf16(pp.x, pp.y) : pack_f16(pp.x, pp.y);
           }
           tmem_st16(sp + c * 16, pk);
+          if (TILES == 2 && c == 1) release(&sh.p_half[t]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[spos.slot]));
+        release(&sh.p_full[spos.slot]);
         const float2 rsum = __fadd2_rn(__fadd2_rn(rs[0], rs[1]), __fadd2_rn(rs[2], rs[3]));
         l += rsum.x + rsum.y;
+      }
+      ++seen;
+      if (TILES == 1) {
         last_pv = spos;
-        spos.step(NB);
-      }
-      if (!ok) break;
-      uint32_t ov[D];
-      if (it.blk.n > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.o_full), items_done & 1u, abort_flag,
-                                               err, kErrWaitSoftmax));
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-          tmem_ld32(o_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(ov + c * 32));
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.o_free));
-        ++items_done;
+        spos.step(kFwdSBufs);
       } else {
-#pragma unroll
-        for (int i = 0; i < D; ++i) ov[i] = 0u;
+        ++blocks;
       }
+    }
+    if (!ok) break;
+    // ------------------------------------------------------------ epilogue
+    uint32_t ov[D];
+    if (seen > 0) {
+      ok = wait(&sh.o_full[t], outs & 1u);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        tmem_ld32(o_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(ov + c * 32));
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.o_free[t]));
+      ++outs;
+    } else {
+#pragma unroll
+      for (int e = 0; e < D; ++e) ov[e] = 0u;
+    }
+    const int head = s.h * g.g + row_head;
+    auto lse_at = [&](int64_t r, int tok, int hd) {
+      return (PAGED ? r : static_cast<int64_t>(s.b) * g.q_len + tok) *
+                 (static_cast<int64_t>(g.heads_kv) * g.g) + hd;
+    };
+    if (!STREAM || s.whole) {
       if (live) {
-        const int64_t r = it.seq.row0 + token;
-        const int head = it.h * g.g + row_head;
-        if (args.lse) {
-          const int64_t at = (PAGED ? r : static_cast<int64_t>(it.b) * g.q_len + token) *
-                                 (static_cast<int64_t>(g.heads_kv) * g.g) + head;
-          args.lse[at] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
-        }
+        const int64_t r = s.seq.row0 + token;
+        if (args.lse)
+          args.lse[lse_at(r, token, head)] =
+              l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
         const float inv_l = l == 0.f ? 0.f : 1.0f / l;
-        T* orow = static_cast<T*>(args.out) + (PAGED ? 0 : it.b * args.o_batch) +
+        T* orow = static_cast<T*>(args.out) + (PAGED ? 0 : s.b * args.o_batch) +
                   r * args.o_token + head * args.o_head;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
           uint32_t pk[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float lo = __uint_as_float(ov[c * 8 + 2 * i]) * inv_l;
-            const float hi = __uint_as_float(ov[c * 8 + 2 * i + 1]) * inv_l;
-            pk[i] = FMT == 1 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+          for (int e = 0; e < 4; ++e) {
+            const float lo = __uint_as_float(ov[c * 8 + 2 * e]) * inv_l;
+            const float hi = __uint_as_float(ov[c * 8 + 2 * e + 1]) * inv_l;
+            pk[e] = FMT == 1 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
           }
           reinterpret_cast<uint4*>(orow)[c] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
       }
+      continue;
     }
+    if constexpr (STREAM) {
+      // ------------------------------------------------- parts of a cut unit
+      const int64_t part_floats = fwd_part_floats(args.part_rows, D);
+      const int c_first = static_cast<int>(s.line0 / sh.line_len);
+      const int c_last = static_cast<int>((s.line0 + s.blk.n - 1) / sh.line_len);
+      // a CTA has two parts at most: slot 0 of a unit that began before its
+      // stretch, slot 1 of one that goes on behind it
+      auto part_of = [&](int c) {
+        return args.part + (2 * static_cast<int64_t>(c) + (c == c_first ? 1 : 0)) * part_floats;
+      };
+      auto part_ml = [&](float* part) {
+        return reinterpret_cast<float2*>(part + static_cast<int64_t>(args.part_rows) * D);
+      };
+      const int base = t * g.tpt * g.g;  // this tile's rows in a part
+      const int rows = (tile.t1 - tile.t0) * g.g;
+      {
+        // four dims of all rows, then the next four: a warp's stores and the
+        // join's loads are contiguous
+        float* mine = part_of(static_cast<int>(blockIdx.x));
+        if (live) {
+          float4* o4 = reinterpret_cast<float4*>(mine) + base + row;
+          if (seen > 0)
+#pragma unroll
+            for (int c = 0; c < D / 4; ++c)
+              __stcg(o4 + c * args.part_rows,
+                     make_float4(__uint_as_float(ov[4 * c]), __uint_as_float(ov[4 * c + 1]),
+                                 __uint_as_float(ov[4 * c + 2]), __uint_as_float(ov[4 * c + 3])));
+          __stcg(part_ml(mine) + base + row, make_float2(m_used, l));
+        }
+      }
+      __threadfence();
+      fwd_barrier(1 + t);
+      if (row == 0) {
+        unsigned int* cnt = args.arrived + static_cast<int64_t>(s.unit) * TILES + t;
+        const unsigned int before = atomicAdd(cnt, 1u);
+        const bool last = before == static_cast<unsigned int>(c_last - c_first);
+        if (last) atomicExch(cnt, 0u);  // ready for the next launch
+        sh.last[t] = last ? 1 : 0;
+      }
+      fwd_barrier(1 + t);
+      const bool join = *reinterpret_cast<volatile int*>(&sh.last[t]) != 0;
+      if (join) {
+        __threadfence();
+        // maximum and 1 / sum of each row over the parts, in their order
+        if (row < rows) {
+          float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            const float2 ml = __ldcg(part_ml(part_of(c)) + base + row);
+            if (ml.y != 0.f) m = fmaxf(m, ml.x);  // a part without a key says nothing
+          }
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            const float2 ml = __ldcg(part_ml(part_of(c)) + base + row);
+            if (ml.y != 0.f) sum += ml.y * ex2_approx(ml.x - m);
+          }
+          join_ml[t * 128 + row] = make_float2(m, sum == 0.f ? 0.f : 1.0f / sum);
+          if (args.lse) {
+            const int tok = tile.t0 + row / g.g;
+            args.lse[lse_at(s.seq.row0 + tok, tok, s.h * g.g + row % g.g)] =
+                sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+          }
+        }
+        fwd_barrier(1 + t);
+        // kJoin elements (four dims of a row) per thread at a time, whose
+        // loads are all in flight at once
+        constexpr int kJoin = 4;
+        const int total = rows * (D / 4);
+        for (int e0 = row; e0 < total; e0 += 128 * kJoin) {
+          float4 o[kJoin];
+          int r[kJoin], x[kJoin];
+          float m[kJoin];
+#pragma unroll
+          for (int u = 0; u < kJoin; ++u) {
+            const int e = e0 + u * 128;
+            r[u] = e < total ? e % rows : -1;
+            x[u] = e / rows;
+            m[u] = r[u] >= 0 ? join_ml[t * 128 + r[u]].x : 0.f;
+            o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            float* part = part_of(c);
+#pragma unroll
+            for (int u = 0; u < kJoin; ++u) {
+              if (r[u] < 0) continue;
+              const float2 ml = __ldcg(part_ml(part) + base + r[u]);
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + base + r[u] +
+                                      x[u] * args.part_rows);
+              if (ml.y != 0.f) {
+                const float f = ex2_approx(ml.x - m[u]);
+                o[u].x += v.x * f;
+                o[u].y += v.y * f;
+                o[u].z += v.z * f;
+                o[u].w += v.w * f;
+              }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kJoin; ++u) {
+            if (r[u] < 0) continue;
+            const float inv = join_ml[t * 128 + r[u]].y;
+            T* orow = static_cast<T*>(args.out) +
+                      (s.seq.row0 + tile.t0 + r[u] / g.g) * args.o_token +
+                      (s.h * g.g + r[u] % g.g) * args.o_head;
+            const uint32_t lo = FMT == 1 ? pack_bf16(o[u].x * inv, o[u].y * inv)
+                                         : pack_f16(o[u].x * inv, o[u].y * inv);
+            const uint32_t hi = FMT == 1 ? pack_bf16(o[u].z * inv, o[u].w * inv)
+                                         : pack_f16(o[u].z * inv, o[u].w * inv);
+            reinterpret_cast<uint2*>(orow)[x[u]] = make_uint2(lo, hi);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
+__global__ void __launch_bounds__(128 + 128 * TILES, 1)
+    attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q,
+                    const __grid_constant__ CUtensorMap tma_k,
+                    const __grid_constant__ CUtensorMap tma_v,
+                    const __grid_constant__ FwdArgs args) {
+  using G = FwdGeom<D>;
+  constexpr int NB = TILES == 1 ? kFwdSBufs : 2;
+  static_assert(TILES * D + NB * kOpsBN <= 512, "TMEM holds 512 columns");
+
+  __shared__ FwdShared sh;
+  __shared__ float2 join_ml[STREAM ? TILES * 128 : 1];
+  extern __shared__ uint8_t dyn_smem[];
+  const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
+  const uint32_t q_smem = base;
+  const uint32_t k_smem = q_smem + TILES * G::Q_BYTES;
+  const uint32_t v_smem = k_smem + args.stages * G::KV_BYTES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&sh.q_full), 1);
+    mbar_init(smem_u32(&sh.q_empty), 1);
+    for (int s = 0; s < args.stages; ++s) {
+      mbar_init(smem_u32(&sh.k_full[s]), 1);
+      mbar_init(smem_u32(&sh.k_empty[s]), 1);
+      mbar_init(smem_u32(&sh.v_full[s]), 1);
+      mbar_init(smem_u32(&sh.v_empty[s]), 1);
+      mbar_init(smem_u32(&sh.v_clean[s]), 1);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(smem_u32(&sh.s_full[b]), 1);
+      mbar_init(smem_u32(&sh.p_full[b]), 4);
+      mbar_init(smem_u32(&sh.pv_done[b]), 1);
+    }
+    for (int t = 0; t < TILES; ++t) {
+      mbar_init(smem_u32(&sh.p_half[t]), 4);
+      mbar_init(smem_u32(&sh.o_full[t]), 1);
+      mbar_init(smem_u32(&sh.o_free[t]), 4);
+    }
+    mbar_init(smem_u32(&sh.drain), 1);
+    sh.abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tma_q);
+    tma_prefetch_desc(&tma_k);
+    tma_prefetch_desc(&tma_v);
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32(&sh.tmem_base), 512);
+    tmem_relinquish();
+  }
+  if constexpr (STREAM) fwd_stretch<PAGED, TILES>(args, sh);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+
+  if (warp < 4) {
+    if constexpr (TILES == 2) fwd_regs_dec<kFwdLowRegs>();
+    if (warp == 0 || warp == 3)
+      fwd_producer<D, PAGED, STREAM, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
+                                            warp == 0 ? k_smem : v_smem, warp == 0, lane);
+    else if (warp == 1 && lane == 0)
+      fwd_mma<FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
+  } else {
+    if constexpr (TILES == 2) fwd_regs_inc<kFwdHighRegs>();
+    fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, join_ml, tmem, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -492,46 +984,98 @@ bool encode_keys_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, i
   return encode_ops_map(map, dtype, t.ptr, 4, dims, strides, box);
 }
 
-template <typename T, int FMT, int D, bool PAGED>
-static gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
+namespace {
+
+// Two tiles per unit where a sequence can fill them.
+int fwd_tiles(const AttnGeom& g) { return g.q_len > g.tpt ? 2 : 1; }
+
+int fwd_spans(const AttnGeom& g) {
+  return static_cast<int>(cdiv(static_cast<uint64_t>(g.q_len),
+                               static_cast<uint64_t>(fwd_tiles(g)) * g.tpt));
+}
+
+// Units are cut where whole ones would leave SMs idle in the last round:
+// fewer than eight rounds of them.
+bool fwd_is_cut(const AttnGeom& g) {
+  const int64_t pairs = static_cast<int64_t>(fwd_spans(g)) * g.batch;
+  return pairs <= kFwdStreamPairs && pairs * g.heads_kv < 8 * kFwdMaxCtas;
+}
+
+int fwd_part_rows(const AttnGeom& g) {
+  return std::min(fwd_tiles(g) * g.tpt, g.q_len) * g.g;
+}
+
+// Counters come first and have a fixed size, so that calls of one plan with
+// different batches agree on where they are (and that they are zero).
+uint64_t fwd_counter_bytes(const AttnGeom& g) {
+  return (static_cast<uint64_t>(8 * kFwdMaxCtas) + g.heads_kv) * 2u * sizeof(unsigned int);
+}
+
+template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
+gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
+  const AttnGeom& g = p.geom;
   CUtensorMap mq, mk, mv;
-  if (!encode_rows_map(&mq, p.dtype, p.q, D, p.geom.g, p.geom.tpt) ||
-      !encode_keys_map(&mk, p.dtype, p.k, D, p.geom.box_rows) ||
-      !encode_keys_map(&mv, p.dtype, p.v, D, p.geom.box_rows))
+  if (!encode_rows_map(&mq, p.dtype, p.q, D, g.g, g.tpt) ||
+      !encode_keys_map(&mk, p.dtype, p.k, D, g.box_rows) ||
+      !encode_keys_map(&mv, p.dtype, p.v, D, g.box_rows))
     return GPO_BAD_ARGS;
-  FwdArgs a;
-  a.geom = p.geom;
+  FwdArgs a{};
+  a.geom = g;
   a.out = p.out;
   a.lse = p.lse;
   a.o_batch = p.o_batch;
   a.o_token = p.o_token;
   a.o_head = p.o_head;
   a.scale_log2 = p.scale * 1.4426950408889634f;
+  a.spans = fwd_spans(g);
+  a.stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
   a.err = c.err;
-  const int64_t items = static_cast<int64_t>(p.geom.tiles) * p.geom.batch * p.geom.heads_kv;
+  const int64_t items = static_cast<int64_t>(a.spans) * g.batch * g.heads_kv;
   if (items > (1ll << 31) - 1024) return GPO_BAD_ARGS;
   a.items = static_cast<int>(items);
-  auto kern = attn_fwd_kernel<T, FMT, D, PAGED>;
-  constexpr uint32_t dyn = (128u + 2u * kFwdStages * kOpsBN) * D * 2u + 1024u;
+  const int sms = std::min(c.sm_count > 0 ? c.sm_count : 148, kFwdMaxCtas);
+  int64_t ctas = std::min<int64_t>(items, sms);
+  if (STREAM) {
+    a.arrived = static_cast<unsigned int*>(p.workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) +
+                                      ((fwd_counter_bytes(g) + 255u) & ~255ull));
+    a.part_rows = fwd_part_rows(g);
+    ctas = sms;
+  }
+  auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES>;
+  const uint32_t dyn =
+      (TILES * 128u + 2u * static_cast<uint32_t>(a.stages) * kOpsBN) * D * 2u + 1024u;
   gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
-  const unsigned grid = static_cast<unsigned>(
-      std::min<int64_t>(items, c.sm_count > 0 ? c.sm_count : 148));
-  kern<<<grid, kFwdThreads, dyn, c.stream>>>(mq, mk, mv, a);
+  kern<<<static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream>>>(mq, mk, mv, a);
   return launch_status();
 }
 
-template <bool PAGED>
-static gpo_status run_fwd_type(const AttnProblem& p, const LaunchCtx& c) {
-  if (p.dtype == GPO_BFLOAT16)
-    return p.dim == 128 ? run_fwd<__nv_bfloat16, 1, 128, PAGED>(p, c)
-                        : run_fwd<__nv_bfloat16, 1, 64, PAGED>(p, c);
-  return p.dim == 128 ? run_fwd<__half, 0, 128, PAGED>(p, c)
-                      : run_fwd<__half, 0, 64, PAGED>(p, c);
+template <typename T, int FMT, int D>
+gpo_status run_fwd_form(const AttnProblem& p, const LaunchCtx& c) {
+  const bool two = fwd_tiles(p.geom) == 2;
+  if (!p.paged)
+    return two ? run_fwd<T, FMT, D, false, false, 2>(p, c)
+               : run_fwd<T, FMT, D, false, false, 1>(p, c);
+  if (fwd_is_cut(p.geom))
+    return two ? run_fwd<T, FMT, D, true, true, 2>(p, c) : run_fwd<T, FMT, D, true, true, 1>(p, c);
+  return two ? run_fwd<T, FMT, D, true, false, 2>(p, c) : run_fwd<T, FMT, D, true, false, 1>(p, c);
+}
+
+}  // namespace
+
+uint64_t attn_paged_workspace(const AttnProblem& p) {
+  // whatever part of the plan's sequences and tokens a call has
+  const AttnGeom& g = p.geom;
+  return ((fwd_counter_bytes(g) + 255u) & ~255ull) +
+         2u * kFwdMaxCtas * static_cast<uint64_t>(fwd_part_floats(fwd_part_rows(g), p.dim)) * 4u;
 }
 
 gpo_status launch_attn_forward(const AttnProblem& p, const LaunchCtx& c) {
-  return p.paged ? run_fwd_type<true>(p, c) : run_fwd_type<false>(p, c);
+  if (p.dtype == GPO_BFLOAT16)
+    return p.dim == 128 ? run_fwd_form<__nv_bfloat16, 1, 128>(p, c)
+                        : run_fwd_form<__nv_bfloat16, 1, 64>(p, c);
+  return p.dim == 128 ? run_fwd_form<__half, 0, 128>(p, c) : run_fwd_form<__half, 0, 64>(p, c);
 }
 
 }  // namespace gpo

@@ -462,8 +462,11 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i < c_lo || i >= c_hi) pr[i] = 0.f;
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t see = bits_below(c_hi, c) & ~bits_below(c_lo, c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pr[c * 32 + i] = (see & (1u << i)) ? pr[c * 32 + i] : 0.f;
+          }
         }
         {
           uint32_t pk[32];
@@ -502,8 +505,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           // 0 * (dP - delta) is not 0 when the masked dP is not finite
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            if (2 * i < c_lo || 2 * i >= c_hi) pk[i] &= 0xffff0000u;
-            if (2 * i + 1 < c_lo || 2 * i + 1 >= c_hi) pk[i] &= 0x0000ffffu;
+            const uint32_t see = (bits_below(c_hi, i / 16) & ~bits_below(c_lo, i / 16)) >>
+                                 (2 * (i % 16));
+            pk[i] &= ((see & 1u) ? 0x0000ffffu : 0u) | ((see & 2u) ? 0xffff0000u : 0u);
           }
         }
         tmem_st32(dp_t, pk);
@@ -782,14 +786,16 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           tmem_ld32(dp_t + c * 32, dp);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float a = pr[c * 32 + i] * (__uint_as_float(dp[i]) - delta);
-            float b = pr[c * 32 + i + 1] * (__uint_as_float(dp[i + 1]) - delta);
-            if (masked) {
-              if (!rm.sees(c * 32 + i)) a = 0.f;
-              if (!rm.sees(c * 32 + i + 1)) b = 0.f;
-            }
-            pk[c * 16 + i / 2] = pack2<FMT>(a, b);
+          for (int i = 0; i < 32; i += 2)
+            pk[c * 16 + i / 2] =
+                pack2<FMT>(pr[c * 32 + i] * (__uint_as_float(dp[i]) - delta),
+                           pr[c * 32 + i + 1] * (__uint_as_float(dp[i + 1]) - delta));
+          if (masked) {
+            const uint32_t see = rm.word(c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              pk[c * 16 + i] &= ((see & (1u << (2 * i))) ? 0x0000ffffu : 0u) |
+                                ((see & (2u << (2 * i))) ? 0xffff0000u : 0u);
           }
         }
         tmem_st32(s_t, pk);

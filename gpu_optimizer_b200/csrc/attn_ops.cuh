@@ -32,7 +32,7 @@ struct AttnGeom {
   int batch, q_len, kv_len;  // q_len: dense length, or the most a sequence has
   int tokens;                // paged: rows of q
   int heads_kv, g, tpt;
-  int tiles;                 // query tiles per sequence (of the longest one)
+  int tiles;                 // dense: query tiles per sequence
   int window, sinks;
 };
 
@@ -90,15 +90,24 @@ __device__ __forceinline__ AttnBlocks attn_blocks(const AttnGeom& g, const AttnS
   return b;
 }
 
-// Keys of a block that a row at position p sees: i <= hi and
-// (i >= lo or i < sink), i counted from the block's first key.
+// Bits [a, b) of word c of a 32-bit mask row (bit i of word c is index 32c + i).
+__device__ __forceinline__ uint32_t bits_below(int n, int c) {
+  const int k = n - 32 * c;
+  return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+}
+
+// Keys of a block that a row at position p sees: i <= p - key0 and
+// (i > p - key0 - window or i < sinks - key0), i counted from the block's
+// first key; as mask words, which cost a test and a select per score.
 struct RowMask {
-  int hi, lo, sink;
-  __device__ __forceinline__ bool sees(int i) const { return i <= hi && (i >= lo || i < sink); }
+  int end, lo, sink;
+  __device__ __forceinline__ uint32_t word(int c) const {
+    return bits_below(end, c) & (~bits_below(lo, c) | bits_below(sink, c));
+  }
 };
 
 __device__ __forceinline__ RowMask row_mask(const AttnGeom& g, int p, int key0) {
-  return RowMask{p - key0, p - g.window + 1 - key0, g.sinks - key0};
+  return RowMask{p - key0 + 1, p - g.window + 1 - key0, g.sinks - key0};
 }
 
 // Whether some row of tokens [t0, t1) misses a key of the block.
@@ -151,6 +160,7 @@ struct AttnProblem {
   void* out;
   int64_t o_batch, o_token, o_head;
   float* lse;
+  void* workspace;  // paged
 };
 
 // What the gradient adds to a dense problem.
@@ -162,6 +172,7 @@ struct AttnGradProblem {
 
 uint64_t attn_grad_workspace(const AttnProblem& p);
 gpo_status launch_attn_grad(const AttnProblem& p, const AttnGradProblem& gp, const LaunchCtx& c);
+uint64_t attn_paged_workspace(const AttnProblem& p);
 gpo_status launch_attn_forward(const AttnProblem& p, const LaunchCtx& c);
 gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c);
 

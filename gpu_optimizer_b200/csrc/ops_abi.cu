@@ -122,7 +122,8 @@ gpo_status refuse(const Refusal& r, char* log, size_t cap) {
   return r.status;
 }
 
-bool paged_problem(const gpo_paged_args& a, bool attention, AttnProblem& p, Refusal& r) {
+bool paged_problem(const gpo_paged_args& a, bool pointers, bool attention, AttnProblem& p,
+                   Refusal& r) {
   if (!check_common(a.dtype, a.head_dim, a.heads_q, a.heads_kv, a.window, a.sinks, a.scale, r))
     return false;
   if (a.reserved != 0) return r.no(GPO_BAD_ARGS, "reserved must be 0");
@@ -160,7 +161,7 @@ bool paged_problem(const gpo_paged_args& a, bool attention, AttnProblem& p, Refu
   p.dim = a.head_dim;
   p.paged = true;
   p.scale = a.scale != 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(a.head_dim));
-  if (a.num_seqs == 0 || a.tokens == 0) return true;
+  if (!pointers || a.num_seqs == 0 || a.tokens == 0) return true;
   if (!a.q_start || !a.kv_len || (a.table_width > 0 && !a.page_table))
     return r.no(GPO_BAD_ARGS, "page_table, q_start or kv_len is null");
   if (a.num_pages > 0) {
@@ -302,8 +303,17 @@ gpo_status gpo_window_attention_grad(const gpo_window_args* a, void* stream, cha
 
 gpo_status gpo_paged_workspace(const gpo_paged_args* a, uint64_t* bytes, char* log, size_t cap) {
   if (!a || !bytes) return GPO_BAD_ARGS;
-  *bytes = 0;
-  return GPO_OK;
+  try {
+    write_log(log, cap, "");
+    *bytes = 0;
+    AttnProblem p{};
+    Refusal r;
+    if (!paged_problem(*a, false, false, p, r)) return refuse(r, log, cap);
+    *bytes = attn_paged_workspace(p);
+    return GPO_OK;
+  } catch (...) {
+    return GPO_INTERNAL;
+  }
 }
 
 gpo_status gpo_paged_attention(const gpo_paged_args* a, void* stream, char* log, size_t cap) {
@@ -312,8 +322,16 @@ gpo_status gpo_paged_attention(const gpo_paged_args* a, void* stream, char* log,
     write_log(log, cap, "");
     AttnProblem p{};
     Refusal r;
-    if (!paged_problem(*a, true, p, r)) return refuse(r, log, cap);
+    if (!paged_problem(*a, true, true, p, r)) return refuse(r, log, cap);
     if (a->num_seqs == 0 || a->tokens == 0 || p.geom.q_len == 0) return GPO_OK;
+    const uint64_t need = attn_paged_workspace(p);
+    if (!a->workspace || a->workspace_bytes < need ||
+        (reinterpret_cast<uintptr_t>(a->workspace) & 255u)) {
+      r.no(GPO_BAD_ARGS, "workspace must be 256-byte aligned and hold " + std::to_string(need) +
+                             " bytes, got " + std::to_string(a->workspace_bytes));
+      return refuse(r, log, cap);
+    }
+    p.workspace = a->workspace;
     return guarded(stream, log, cap, [&](LaunchCtx& c) { return launch_attn_forward(p, c); });
   } catch (...) {
     return GPO_INTERNAL;
@@ -326,7 +344,7 @@ gpo_status gpo_cache_append(const gpo_paged_args* a, void* stream, char* log, si
     write_log(log, cap, "");
     AttnProblem p{};
     Refusal r;
-    if (!paged_problem(*a, false, p, r)) return refuse(r, log, cap);
+    if (!paged_problem(*a, true, false, p, r)) return refuse(r, log, cap);
     if (a->num_seqs == 0 || a->tokens == 0 || a->num_pages == 0) return GPO_OK;
     return guarded(stream, log, cap, [&](LaunchCtx& c) { return launch_cache_append(p, c); });
   } catch (...) {
