@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
     if (warp == 0 || warp == 3)
       fwd_producer<D, PAGED, STREAM, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
                                             warp == 0 ? k_smem : v_smem, warp == 0, lane);
-    else if (warp == 1 && lane == 0)
+    else if (warp == 1 && elect_one())
       fwd_mma<FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
   } else {
     if constexpr (TILES == 2) fwd_regs_inc<kFwdHighRegs>();

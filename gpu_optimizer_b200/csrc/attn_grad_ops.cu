@@ -7,21 +7,36 @@
 //   dQ = scale dS K                  dK = scale dS^T Q
 // with dK and dV summed over the query heads of a kv head.
 //
-// Three kernels: the rows' statistics (memory bound), dK and dV by key tile
-// and dQ by query tile.  The scores are computed in both of the latter (7
-// products in place of 5), because each sum then has one owner and a fixed
-// order: no atomics, equal inputs give equal bits, and no fp32 copy of dQ
+// Two kernels: the rows' statistics (memory bound), and one persistent
+// kernel that first works through the key tiles (dK, dV) and then through
+// the query tiles (dQ).  The scores are computed in both (7 products in
+// place of 5), because each sum then has one owner and a fixed order: no
+// atomics on values, equal inputs give equal bits, and no fp32 copy of dQ
 // goes through memory.  P and dS are rounded to the inputs' type as MMA
-// operands; every sum is fp32 in TMEM.
+// operands; every sum is fp32 in TMEM.  (A third, small kernel joins the
+// sink keys' partial sums, see kv_piece.)
+//
+// Roles of the persistent kernel, one CTA per SM:
+//   warp 0     takes work items from a counter; TMA of the item's first own
+//              tile (K or Q), of ring A (Q or K) and of the row statistics
+//   warp 3     TMA of the second own tile (V or dO) and of ring B (dO or V)
+//   warp 1     MMA issuer
+//   warp 2     TMEM owner
+//   warps 4-11 elementwise: thread = TMEM lane, 64 of a tile's 128 columns
+// Ring A is three tiles deep and ring B two (with D = 128 that fills shared
+// memory): a tile of A is needed by the last product of a step and again
+// missing at the first product of the next but one, so with two slots the
+// MMA warp waited 2000 cycles per step for it.
 #include <algorithm>
 
 #include "attn_ops.cuh"
 
 namespace gpo {
 
-constexpr int kGradStages = 2;
-constexpr int kGradThreads = 384;  // 4 service warps, 2 x 4 elementwise warps
+constexpr int kGradA = 3, kGradB = 2;  // ring depths
+constexpr int kGradThreads = 384;      // 4 service warps, 2 x 4 elementwise warps
 constexpr int kGradEwWarps = 8;
+constexpr int kGradReaders = 2 + kGradEwWarps;  // of an item: warp 3, warp 1, elementwise
 
 struct GradArgs {
   AttnGeom geom;
@@ -40,7 +55,8 @@ struct GradArgs {
   int sink_tiles;  // of them, tiles with a sink key
   int far_tiles;   // query tiles of a far piece (see kv_piece)
   int far_pieces;  // far pieces of a sink tile
-  int items;
+  int kv_items, items;     // items [0, kv_items): key tiles, then query tiles
+  unsigned int* next;      // counter of items, zeroed by the statistics kernel
   unsigned int* err;
 };
 
@@ -54,6 +70,8 @@ __device__ __forceinline__ float* grad_stats(const GradArgs& a, int b, int h, in
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) {
   const AttnGeom& g = a.geom;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.next = 0u;
+  if (g.tiles == 0) return;
   constexpr int LPR = D / 8, RPW = 32 / LPR;  // lanes per row, rows per warp
   const int tile = blockIdx.x % g.tiles, bh = blockIdx.x / g.tiles;
   const int h = bh % g.heads_kv, b = bh / g.heads_kv;
@@ -95,45 +113,83 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
 
 // ------------------------------------------------------------- shared parts
 struct GradShared {
-  uint64_t own_full, own_empty;                            // the item's own two tiles
-  uint64_t in_full[kGradStages], in_empty[kGradStages];    // ring of the other side
-  uint64_t s_full[2], dp_full;
+  uint64_t own_full[2], own_empty[2];
+  uint64_t a_full[kGradA], a_empty[kGradA];
+  uint64_t b_full[kGradB], b_empty[kGradB];
+  uint64_t st_full[2], st_empty[2];  // row statistics (key tiles)
+  uint64_t s_full[2], dp_full;       // key tiles use s_full[0] alone
+  uint64_t q_s_full[2];              // the two S buffers of query tiles
   uint64_t p_ready, ds_ready;
   uint64_t acc_full, acc_free;
+  uint64_t item_full[2], item_empty[2];
   uint64_t drain;
+  int item[2];
   uint32_t tmem_base;
   int abort;
 };
 
+template <int D>
+struct GradGeom {
+  static constexpr uint32_t TILE = 128u * D * 2;  // bytes of a 128-row tile
+  static constexpr uint32_t OWN = 0;
+  static constexpr uint32_t RING_A = 2 * TILE;
+  static constexpr uint32_t RING_B = RING_A + kGradA * TILE;
+  static constexpr uint32_t STATS = RING_B + kGradB * TILE;
+  static constexpr uint32_t SHARED = STATS + 2 * 1024u;
+  static constexpr uint32_t BYTES = SHARED + sizeof(GradShared);
+  static_assert(BYTES <= kMaxSmemPerCta, "shared memory");
+};
+
 __device__ __forceinline__ void grad_init(GradShared& sh) {
-  mbar_init(smem_u32(&sh.own_full), 1);
-  mbar_init(smem_u32(&sh.own_empty), 1);
-  for (int s = 0; s < kGradStages; ++s) {
-    mbar_init(smem_u32(&sh.in_full[s]), 1);
-    mbar_init(smem_u32(&sh.in_empty[s]), 1);
-  }
-  mbar_init(smem_u32(&sh.s_full[0]), 1);
-  mbar_init(smem_u32(&sh.s_full[1]), 1);
-  mbar_init(smem_u32(&sh.dp_full), 1);
-  mbar_init(smem_u32(&sh.p_ready), kGradEwWarps);
-  mbar_init(smem_u32(&sh.ds_ready), kGradEwWarps);
-  mbar_init(smem_u32(&sh.acc_full), 1);
-  mbar_init(smem_u32(&sh.acc_free), kGradEwWarps);
-  mbar_init(smem_u32(&sh.drain), 1);
+  auto init = [](uint64_t* b, int n, uint32_t count) {
+    for (int i = 0; i < n; ++i) mbar_init(smem_u32(b + i), count);
+  };
+  init(sh.own_full, 2, 1);
+  init(sh.own_empty, 2, 1);
+  init(sh.a_full, kGradA, 1);
+  init(sh.a_empty, kGradA, 1);
+  init(sh.b_full, kGradB, 1);
+  init(sh.b_empty, kGradB, 1);
+  init(sh.st_full, 2, 1);
+  init(sh.st_empty, 2, kGradEwWarps);
+  init(sh.s_full, 2, 1);
+  init(&sh.dp_full, 1, 1);
+  init(sh.q_s_full, 2, 1);
+  init(&sh.p_ready, 1, kGradEwWarps);
+  init(&sh.ds_ready, 1, kGradEwWarps);
+  init(&sh.acc_full, 1, 1);
+  init(&sh.acc_free, 1, kGradEwWarps);
+  init(sh.item_full, 2, 1);
+  init(sh.item_empty, 2, kGradReaders);
+  init(&sh.drain, 1, 1);
   sh.abort = 0;
   fence_barrier_init();
 }
 
+template <int N>
 struct GradRing {
   int slot = 0;
   uint32_t parity = 0;
   __device__ __forceinline__ void step() {
-    if (++slot == kGradStages) {
+    if (++slot == N) {
       slot = 0;
       parity ^= 1u;
     }
   }
 };
+
+// The item of the CTA's it-th turn, published by warp 0 (-1: no more).
+template <bool WARP>
+__device__ __forceinline__ bool grad_next_item(GradShared& sh, int it, volatile int* abort_flag,
+                                               unsigned int* err, uint32_t site, int& item) {
+  bool ok = mbar_wait(smem_u32(&sh.item_full[it & 1]), (it >> 1) & 1u, abort_flag, err, site);
+  if (WARP) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  item = *reinterpret_cast<volatile int*>(&sh.item[it & 1]);
+  if (WARP) __syncwarp();
+  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sh.item_empty[it & 1]));
+  return true;
+}
 
 // D[tmem, 128 x N] (+)= A B^T over 128-byte-swizzled K-major tiles of 128
 // rows and D dims (both operands in shared memory).
@@ -236,27 +292,539 @@ __device__ __forceinline__ float* kv_partial(const GradArgs& a, int b, int h, in
   return a.partial + (row * (1 + a.far_pieces) + piece) * (2 * D);
 }
 
-template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kGradThreads, 1)
-    attn_grad_kv_kernel(const __grid_constant__ CUtensorMap tma_q,
-                        const __grid_constant__ CUtensorMap tma_do,
-                        const __grid_constant__ CUtensorMap tma_k,
-                        const __grid_constant__ CUtensorMap tma_v,
-                        const __grid_constant__ GradArgs args) {
-  constexpr uint32_t TILE = 128u * D * 2;        // bytes of a 128-row tile
-  constexpr uint32_t STAGE = 2 * TILE + 1024u;   // Q, dO, statistics
-  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128, false, false);
-  constexpr uint32_t IDESC_O = make_idesc(FMT, 128, D, false, true);
-  constexpr uint32_t S_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
+// ------------------------------------------------------------ query tiles
+struct QItem {
+  int b, h, t0, t1, tile;
+  AttnSeq seq;
+  AttnBlocks blk;
+};
 
-  __shared__ GradShared sh;
-  extern __shared__ uint8_t dyn_smem[];
-  const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
-  const uint32_t k_smem = base, v_smem = base + TILE, ring = base + 2 * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ QItem q_item(const GradArgs& a, int item) {
+  const AttnGeom& g = a.geom;
+  QItem it;
+  const int r = (item - a.kv_items) / g.heads_kv;
+  it.h = (item - a.kv_items) % g.heads_kv;
+  it.b = r % g.batch;
+  it.tile = g.tiles - 1 - r / g.batch;  // the longest rows first
+  it.seq = AttnSeq{g.q_len, g.kv_len, 0, g.kv_len - g.q_len};
+  it.t0 = it.tile * g.tpt;
+  it.t1 = min(it.t0 + g.tpt, g.q_len);
+  it.blk = attn_blocks(g, it.seq, it.t0, it.t1);
+  return it;
+}
+
+struct GradMaps {
+  const CUtensorMap *q, *dout, *k, *v;
+};
+
+// ---------------------------------------------------------------- producers
+// Side 0: own tile K (key tiles) or Q, ring A of Q + statistics, or of K.
+// Side 1: own tile V or dO, ring B of dO or V.
+template <int D, int SIDE>
+__device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& sh,
+                                              const GradMaps& maps, uint32_t base) {
+  using G = GradGeom<D>;
+  constexpr int N = SIDE == 0 ? kGradA : kGradB;
   const AttnGeom& g = args.geom;
   unsigned int* err = args.err;
+  volatile int* abort_flag = &sh.abort;
+  const uint32_t own_smem = base + G::OWN + SIDE * G::TILE;
+  const uint32_t ring = base + (SIDE == 0 ? G::RING_A : G::RING_B);
+  uint64_t* full = SIDE == 0 ? sh.a_full : sh.b_full;
+  uint64_t* empty = SIDE == 0 ? sh.a_empty : sh.b_empty;
+  const uint32_t rows_bytes = static_cast<uint32_t>(g.tpt * g.g) * D * 2;
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    return mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitProducer);
+  };
+  // 128 keys from `row`, or the rows of a query tile
+  auto load_keys = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int h, int row, int b) {
+    mbar_arrive_expect_tx(smem_u32(bar), G::TILE);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_4d(dst + c * 128 * 128, m, smem_u32(bar), c * 64, h, row, b);
+  };
+  auto load_rows = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int h, int token,
+                       int b) {
+    mbar_arrive_expect_tx(smem_u32(bar), rows_bytes);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_load_5d(dst + c * 128 * 128, m, smem_u32(bar), c * 64, 0, h, token, b);
+  };
+  bool ok = true;
+  int own = 0, issued = 0, stats = 0;
+  GradRing<N> pos;
+  GradRing<2> st;
+  for (int it = 0; ok; ++it) {
+    int item;
+    if constexpr (SIDE == 0) {
+      // the slot's last item has been read by every other role
+      if (it >= 2 && !wait(&sh.item_empty[it & 1], ((it >> 1) - 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      const int next = static_cast<int>(atomicAdd(args.next, 1u));
+      item = next < args.items ? next : -1;
+      sh.item[it & 1] = item;
+      mbar_arrive(smem_u32(&sh.item_full[it & 1]));
+    } else {
+      ok = grad_next_item<false>(sh, it, abort_flag, err, kErrWaitProducer, item);
+    }
+    if (!ok || item < 0) break;
+    const bool keys = item < args.kv_items;
+    KvPiece p{};
+    QItem qi{};
+    if (keys)
+      p = kv_piece(args, item);
+    else
+      qi = q_item(args, item);
+    const int n = keys ? p.n : qi.blk.n;
+    if (n == 0) continue;
+    if (own > 0 && !wait(&sh.own_empty[SIDE], (own - 1) & 1u)) {
+      ok = false;
+      break;
+    }
+    if (keys)
+      load_keys(own_smem, SIDE == 0 ? maps.k : maps.v, &sh.own_full[SIDE], p.h, p.kt * 128, p.b);
+    else
+      load_rows(own_smem, SIDE == 0 ? maps.q : maps.dout, &sh.own_full[SIDE], qi.h, qi.t0, qi.b);
+    ++own;
+    for (int j = 0; j < n; ++j) {
+      if (!wait(&empty[pos.slot], pos.parity ^ 1u)) {
+        ok = false;
+        break;
+      }
+      const uint32_t dst = ring + pos.slot * G::TILE;
+      if (keys)
+        load_rows(dst, SIDE == 0 ? maps.q : maps.dout, &full[pos.slot], p.h,
+                  (p.first + j) * g.tpt, p.b);
+      else
+        load_keys(dst, SIDE == 0 ? maps.k : maps.v, &full[pos.slot], qi.h, qi.blk.at(j) * 128,
+                  qi.b);
+      ++issued;
+      pos.step();
+      if (SIDE == 0 && keys) {
+        if (!wait(&sh.st_empty[st.slot], st.parity ^ 1u)) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = smem_u32(&sh.st_full[st.slot]);
+        mbar_arrive_expect_tx(bar, 1024u);
+        bulk_load(base + G::STATS + st.slot * 1024u, grad_stats(args, p.b, p.h, p.first + j),
+                  1024u, bar);
+        ++stats;
+        st.step();
+      }
+    }
+  }
+  if (!ok) {
+    // let the copies in flight land before the CTA can exit
+    if (own > 0) mbar_wait_drain(smem_u32(&sh.own_full[SIDE]), (own - 1) & 1u, err);
+    for (int j = max(0, issued - N); j < issued; ++j)
+      mbar_wait_drain(smem_u32(&full[j % N]), (j / N) & 1u, err);
+    for (int j = max(0, stats - 2); j < stats; ++j)
+      mbar_wait_drain(smem_u32(&sh.st_full[j & 1]), (j >> 1) & 1u, err);
+  }
+}
 
+// -------------------------------------------------------------- MMA issuer
+// Key tiles: S(j+1) follows dV(j), which reads P(j) in the same columns, and
+// dP(j+1) follows dK(j) in the same way: MMAs run in issue order.
+// Query tiles: S(j+1) goes to the other buffer before dS(j) is waited for;
+// dP(j+1) then has its columns back and comes before dQ(j), so that the
+// elementwise warps wait least.
+template <int D>
+struct GradTmem {
+  // key tiles: S^T and P^T, dP^T and dS^T, dV, dK
+  static constexpr uint32_t S = 0, DP = 128, DV = 256, DK = 256 + D;
+  // query tiles: two S buffers (dS overlays S), dP, dQ
+  static constexpr uint32_t QS = 0, QDP = 256, DQ = 384;
+};
+
+template <int FMT, int D>
+__device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, uint32_t base,
+                                         uint32_t tmem) {
+  using G = GradGeom<D>;
+  using C = GradTmem<D>;
+  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128, false, false);
+  constexpr uint32_t IDESC_O = make_idesc(FMT, 128, D, false, true);
+  unsigned int* err = args.err;
+  volatile int* abort_flag = &sh.abort;
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    const uint32_t b = smem_u32(bar);
+    return mbar_test_wait(b, parity) || mbar_wait(b, parity, abort_flag, err, kErrWaitMma);
+  };
+  auto commit = [&](const uint64_t* bar) { mma_commit(smem_u32(bar)); };
+  const uint32_t own0 = smem_desc_lo(base + G::OWN, 16);
+  const uint32_t own1 = smem_desc_lo(base + G::OWN + G::TILE, 16);
+  // descriptors of a ring tile as rows (K-major) and as columns (MN-major)
+  auto rows_of = [&](uint32_t ring, int slot) {
+    return smem_desc_lo(base + ring + slot * G::TILE, 16);
+  };
+  auto cols_of = [&](uint32_t ring, int slot) {
+    return smem_desc_lo(base + ring + slot * G::TILE, 128 * 128);
+  };
+  bool ok = true, was_keys = true;
+  GradRing<kGradA> a;  // next tile of ring A that has not been waited for
+  GradRing<kGradB> b;
+  uint32_t own = 0, cnt = 0, qcnt = 0;
+  for (int it = 0; ok; ++it) {
+    int item;
+    ok = grad_next_item<false>(sh, it, abort_flag, err, kErrWaitMma, item);
+    if (!ok || item < 0) break;
+    const bool keys = item < args.kv_items;
+    const int n = keys ? kv_piece(args, item).n : q_item(args, item).blk.n;
+    if (n == 0) continue;
+    const uint32_t op = own & 1u;
+    if (keys) {
+      ok = wait(&sh.own_full[0], op) && wait(&sh.a_full[a.slot], a.parity);
+      if (!ok) break;
+      mma_rows<D>(tmem + C::S, own0, rows_of(G::RING_A, a.slot), IDESC_S);
+      commit(&sh.s_full[0]);
+      if (n == 1) commit(&sh.own_empty[0]);
+      ok = wait(&sh.own_full[1], op) && wait(&sh.b_full[b.slot], b.parity);
+      if (!ok) break;
+      mma_rows<D>(tmem + C::DP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
+      commit(&sh.dp_full);
+      if (n == 1) commit(&sh.own_empty[1]);
+      // the previous item's sums have been read out of TMEM
+      if (own > 0) ok = wait(&sh.acc_free, (own - 1) & 1u);
+      for (int j = 0; j < n && ok; ++j, ++cnt) {
+        const int aj = a.slot, bj = b.slot;
+        const bool more = j + 1 < n;
+        ok = wait(&sh.p_ready, cnt & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        mma_cols(tmem + C::DV, tmem + C::S, cols_of(G::RING_B, bj), IDESC_O, j == 0);
+        commit(&sh.b_empty[bj]);
+        a.step();
+        b.step();
+        if (more) {
+          ok = wait(&sh.a_full[a.slot], a.parity);
+          if (!ok) break;
+          mma_rows<D>(tmem + C::S, own0, rows_of(G::RING_A, a.slot), IDESC_S);
+          commit(&sh.s_full[0]);
+          if (j + 2 == n) commit(&sh.own_empty[0]);
+        }
+        ok = wait(&sh.ds_ready, cnt & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        mma_cols(tmem + C::DK, tmem + C::DP, cols_of(G::RING_A, aj), IDESC_O, j == 0);
+        commit(&sh.a_empty[aj]);
+        if (more) {
+          ok = wait(&sh.b_full[b.slot], b.parity);
+          if (!ok) break;
+          mma_rows<D>(tmem + C::DP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
+          commit(&sh.dp_full);
+          if (j + 2 == n) commit(&sh.own_empty[1]);
+        } else {
+          commit(&sh.acc_full);
+        }
+      }
+    } else {
+      ok = wait(&sh.own_full[0], op) && wait(&sh.a_full[a.slot], a.parity);
+      if (!ok) break;
+      mma_rows<D>(tmem + C::QS + (qcnt & 1u) * 128, own0, rows_of(G::RING_A, a.slot), IDESC_S);
+      commit(&sh.q_s_full[qcnt & 1u]);
+      if (n == 1) commit(&sh.own_empty[0]);
+      ok = wait(&sh.own_full[1], op) && wait(&sh.b_full[b.slot], b.parity);
+      // dP of query tiles has the columns of dV of key tiles
+      const bool turn = was_keys && own > 0;
+      if (ok && turn) ok = wait(&sh.acc_free, (own - 1) & 1u);
+      if (!ok) break;
+      was_keys = false;
+      mma_rows<D>(tmem + C::QDP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
+      commit(&sh.dp_full);
+      commit(&sh.b_empty[b.slot]);
+      b.step();
+      if (n == 1) commit(&sh.own_empty[1]);
+      if (own > 0 && !turn) ok = wait(&sh.acc_free, (own - 1) & 1u);
+      for (int j = 0; j < n && ok; ++j, ++cnt, ++qcnt) {
+        const int aj = a.slot;
+        const bool more = j + 1 < n;
+        a.step();
+        if (more) {
+          ok = wait(&sh.a_full[a.slot], a.parity);
+          if (!ok) break;
+          mma_rows<D>(tmem + C::QS + ((qcnt + 1) & 1u) * 128, own0, rows_of(G::RING_A, a.slot),
+                      IDESC_S);
+          commit(&sh.q_s_full[(qcnt + 1) & 1u]);
+          if (j + 2 == n) commit(&sh.own_empty[0]);
+        }
+        ok = wait(&sh.ds_ready, cnt & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        if (more) {
+          ok = wait(&sh.b_full[b.slot], b.parity);
+          if (!ok) break;
+          mma_rows<D>(tmem + C::QDP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
+          commit(&sh.dp_full);
+          commit(&sh.b_empty[b.slot]);
+          b.step();
+          if (j + 2 == n) commit(&sh.own_empty[1]);
+        }
+        mma_cols(tmem + C::DQ, tmem + C::QS + (qcnt & 1u) * 128, cols_of(G::RING_A, aj), IDESC_O,
+                 j == 0);
+        commit(&sh.a_empty[aj]);
+        if (!more) commit(&sh.acc_full);
+      }
+    }
+    ++own;
+  }
+  if (!ok) {
+    mma_commit(smem_u32(&sh.drain));
+    mbar_wait_drain(smem_u32(&sh.drain), 0, err);
+  }
+}
+
+// ------------------------------------------------------------- elementwise
+template <typename T, int FMT, int D>
+struct GradEw {
+  const GradArgs& args;
+  GradShared& sh;
+  uint32_t base, tmem;
+  int wg, row, lane;
+  uint32_t lane_addr;
+  bool ok = true;
+  GradRing<2> st;
+  uint32_t own = 0, cnt = 0, qcnt = 0;
+
+  __device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity) {
+    return ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &sh.abort, args.err,
+                                                  kErrWaitSoftmax));
+  }
+  // after TMEM stores that a later MMA reads
+  __device__ __forceinline__ void release(uint64_t* bar) {
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(bar));
+  }
+  __device__ __forceinline__ void load64(uint32_t taddr, float (&x)[64]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      tmem_ld32(taddr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(
+                                    reinterpret_cast<uint32_t*>(x) + c * 32));
+    tmem_wait_ld();
+  }
+  __device__ __forceinline__ void acc_release() {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.acc_free));
+    ++own;
+  }
+
+  // thread = key; 64 packed query rows of the tile
+  __device__ __forceinline__ void keys(int item) {
+    using G = GradGeom<D>;
+    using C = GradTmem<D>;
+    const AttnGeom& g = args.geom;
+    const uint32_t s_t = tmem + lane_addr + C::S + wg * 64;
+    const uint32_t dp_t = tmem + lane_addr + C::DP + wg * 64;
+    const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
+    const int off = g.kv_len - g.q_len;
+    const KvPiece p = kv_piece(args, item);
+    const int k0 = p.kt * 128, key = k0 + row;
+    // tokens that see this key: [key - off, key - off + window), or all
+    // later ones for a sink key
+    const int tok_lo = key - off;
+    const int tok_hi = (g.window == kOpsNoWindow || key < g.sinks) ? kOpsMaxLen
+                                                                    : tok_lo + g.window - 1;
+    for (int j = 0; j < p.n; ++j, ++cnt) {
+      const int ta = (p.first + j) * g.tpt, tb = ta + g.tpt - 1;
+      // some key of the tile misses some token of the query tile
+      const bool masked = k0 + 127 - off > ta ||
+                          (g.window != kOpsNoWindow && k0 - off + g.window - 1 < tb);
+      // packed rows of this thread's half that see the key: [c_lo, c_hi)
+      const int c_lo = (max(tok_lo, ta) - ta) * g.g - wg * 64;
+      const int c_hi = (min(tok_hi, tb) - ta + 1) * g.g - wg * 64;
+      if (!wait(&sh.st_full[st.slot], st.parity) || !wait(&sh.s_full[0], cnt & 1u)) return;
+      tc_fence_after();
+      const uint32_t stat = base + G::STATS + st.slot * 1024u + wg * 256;
+      float pr[64];
+      load64(s_t, pr);
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        float4 nl;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(nl.x), "=f"(nl.y), "=f"(nl.z), "=f"(nl.w)
+                     : "r"(stat + i * 4));
+        const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2,
+                                    make_float2(nl.x, nl.y));
+        const float2 y = __ffma2_rn(make_float2(pr[i + 2], pr[i + 3]), scale2,
+                                    make_float2(nl.z, nl.w));
+        pr[i] = ex2_approx(x.x);
+        pr[i + 1] = ex2_approx(x.y);
+        pr[i + 2] = ex2_approx(y.x);
+        pr[i + 3] = ex2_approx(y.y);
+      }
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t see = bits_below(c_hi, c) & ~bits_below(c_lo, c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) pr[c * 32 + i] = (see & (1u << i)) ? pr[c * 32 + i] : 0.f;
+        }
+      }
+      {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) pk[i] = pack2<FMT>(pr[2 * i], pr[2 * i + 1]);
+        tmem_st32(s_t, pk);
+      }
+      release(&sh.p_ready);
+      if (!wait(&sh.dp_full, cnt & 1u)) return;
+      tc_fence_after();
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dp[32];
+        tmem_ld32(dp_t + c * 32, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4 dl;
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(dl.x), "=f"(dl.y), "=f"(dl.z), "=f"(dl.w)
+                       : "r"(stat + 512 + (c * 32 + i) * 4));
+          const float d[4] = {dl.x, dl.y, dl.z, dl.w};
+          float ds[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            ds[u] = pr[c * 32 + i + u] * (__uint_as_float(dp[i + u]) - d[u]);
+          pk[c * 16 + i / 2] = pack2<FMT>(ds[0], ds[1]);
+          pk[c * 16 + i / 2 + 1] = pack2<FMT>(ds[2], ds[3]);
+        }
+      }
+      if (masked) {
+        // 0 * (dP - delta) is not 0 when the masked dP is not finite
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint32_t see = (bits_below(c_hi, i / 16) & ~bits_below(c_lo, i / 16)) >>
+                               (2 * (i % 16));
+          pk[i] &= ((see & 1u) ? 0x0000ffffu : 0u) | ((see & 2u) ? 0xffff0000u : 0u);
+        }
+      }
+      tmem_st32(dp_t, pk);
+      release(&sh.ds_ready);
+      if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
+      st.step();
+    }
+    if (p.n > 0) {
+      if (!wait(&sh.acc_full, own & 1u)) return;
+      tc_fence_after();
+    }
+    // warpgroup 0 writes dV, warpgroup 1 dK
+    const uint32_t acc = tmem + lane_addr + (wg == 0 ? C::DV : C::DK);
+    const float f = wg == 0 ? 1.f : args.scale;
+    const bool sink = key < g.sinks;
+    T* dst = wg == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
+                           p.h * args.dv_head
+                     : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
+                           p.h * args.dk_head;
+    if (k0 < g.sinks) {
+      float* part = sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + wg * D : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(acc + c * 32, r);
+        tmem_wait_ld();
+        if (sink && key < g.kv_len) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(part + c * 32 + i) =
+                p.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                         : make_float4(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f,
+                                       __uint_as_float(r[i + 2]) * f,
+                                       __uint_as_float(r[i + 3]) * f);
+        }
+      }
+    }
+    if (p.piece == 0) store_row<T, FMT, D>(acc, dst, f, key < g.kv_len && !sink, p.n == 0);
+    if (p.n > 0) acc_release();
+  }
+
+  // thread = packed query row; 64 keys of the block
+  __device__ __forceinline__ void rows(int item) {
+    using C = GradTmem<D>;
+    const AttnGeom& g = args.geom;
+    const uint32_t dp_t = tmem + lane_addr + C::QDP + wg * 64;
+    const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
+    const QItem it = q_item(args, item);
+    const int row_token = row / g.g, row_head = row % g.g;
+    const int token = it.t0 + row_token;
+    const bool live = row_token < g.tpt && token < it.t1;
+    const float* stat = grad_stats(args, it.b, it.h, it.tile);
+    const float nl = stat[row], delta = stat[128 + row];
+    const float2 shift2 = make_float2(nl, nl);
+    for (int j = 0; j < it.blk.n; ++j, ++cnt, ++qcnt) {
+      const int key0 = it.blk.at(j) * 128;
+      const bool masked = block_is_masked(g, it.seq, it.t0, it.t1, key0);
+      const RowMask rm = row_mask(g, token + it.seq.off, key0 + wg * 64);
+      const uint32_t s_t = tmem + lane_addr + C::QS + (qcnt & 1u) * 128 + wg * 64;
+      if (!wait(&sh.q_s_full[qcnt & 1u], (qcnt >> 1) & 1u)) return;
+      tc_fence_after();
+      float pr[64];
+      load64(s_t, pr);
+#pragma unroll
+      for (int i = 0; i < 64; i += 2) {
+        const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2, shift2);
+        pr[i] = ex2_approx(x.x);
+        pr[i + 1] = ex2_approx(x.y);
+      }
+      if (!wait(&sh.dp_full, cnt & 1u)) return;
+      tc_fence_after();
+      uint32_t pk[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t dp[32];
+        tmem_ld32(dp_t + c * 32, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          pk[c * 16 + i / 2] = pack2<FMT>(pr[c * 32 + i] * (__uint_as_float(dp[i]) - delta),
+                                          pr[c * 32 + i + 1] * (__uint_as_float(dp[i + 1]) - delta));
+        if (masked) {
+          const uint32_t see = rm.word(c);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            pk[c * 16 + i] &= ((see & (1u << (2 * i))) ? 0x0000ffffu : 0u) |
+                              ((see & (2u << (2 * i))) ? 0xffff0000u : 0u);
+        }
+      }
+      tmem_st32(s_t, pk);
+      release(&sh.ds_ready);
+    }
+    if (it.blk.n > 0) {
+      if (!wait(&sh.acc_full, own & 1u)) return;
+      tc_fence_after();
+    }
+    // each warpgroup writes half of the dims
+    T* dst = static_cast<T*>(args.dq) + it.b * args.dq_batch + token * args.dq_token +
+             (it.h * g.g + row_head) * args.dq_head + wg * (D / 2);
+    store_row<T, FMT, D / 2>(tmem + lane_addr + C::DQ + wg * (D / 2), dst, args.scale, live,
+                             it.blk.n == 0);
+    if (it.blk.n > 0) acc_release();
+  }
+};
+
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(kGradThreads, 1)
+    attn_grad_kernel(const __grid_constant__ CUtensorMap tma_q,
+                     const __grid_constant__ CUtensorMap tma_do,
+                     const __grid_constant__ CUtensorMap tma_k,
+                     const __grid_constant__ CUtensorMap tma_v,
+                     const __grid_constant__ GradArgs args) {
+  using G = GradGeom<D>;
+  extern __shared__ __align__(1024) uint8_t dyn_smem[];
+  const uint32_t base = smem_u32(dyn_smem);
+  GradShared& sh = *reinterpret_cast<GradShared*>(dyn_smem + G::SHARED);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AttnGeom& g = args.geom;
+  if (base & 1023u) {  // the swizzled tiles need the alignment asked for above
+    if (threadIdx.x == 0) atomicOr(args.err, kErrBadLaunch);
+    return;
+  }
+  const GradMaps maps{&tma_q, &tma_do, &tma_k, &tma_v};
   if (threadIdx.x == 0) {
     grad_init(sh);
     tma_prefetch_desc(&tma_q);
@@ -264,16 +832,17 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     tma_prefetch_desc(&tma_k);
     tma_prefetch_desc(&tma_v);
   }
-  // rows of a query tile that hold no query (128 is not a multiple of g):
-  // no copy writes them, and 0 * (what was there) need not be 0
+  // Rows of a query tile that hold no query (128 is not a multiple of g): no
+  // copy writes them, and 0 * (what was there) need not be 0.  Cleared in
+  // the slots that hold query tiles as dK's and dV's operands (key tiles;
+  // query tiles come later and have their rows as the M dimension).
   {
     const int unused = 128 - g.tpt * g.g;
     const int vecs = unused * 8 * (D / 64);
-    for (int i = threadIdx.x; i < kGradStages * 2 * vecs; i += kGradThreads) {
-      const int s = i / (2 * vecs), m = i / vecs % 2, e = i % vecs;
-      const int atom = e / (unused * 8), x = e % (unused * 8);
+    for (int i = threadIdx.x; i < (kGradA + kGradB) * vecs; i += kGradThreads) {
+      const int e = i % vecs, atom = e / (unused * 8), x = e % (unused * 8);
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                       ring + s * STAGE + m * TILE + atom * 128 * 128 +
+                       base + G::RING_A + (i / vecs) * G::TILE + atom * 128 * 128 +
                        (128 - unused) * 128 + x * 16),
                    "r"(0)
                    : "memory");
@@ -288,272 +857,24 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
-  volatile int* abort_flag = &sh.abort;
-
-  if (warp == 0 && lane == 0) {
-    // -------------------------------------------------------- producer
-    const uint32_t rows_bytes = static_cast<uint32_t>(g.tpt * g.g) * D * 2;
-    bool ok = true;
-    int issued = 0, own = 0;
-    GradRing pos;
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const KvPiece p = kv_piece(args, item);
-      if (p.n == 0) continue;
-      ok = own == 0 || mbar_wait(smem_u32(&sh.own_empty), (own - 1) & 1u, abort_flag, err,
-                                 kErrWaitProducer);
-      if (!ok) break;
-      mbar_arrive_expect_tx(smem_u32(&sh.own_full), 2 * TILE);
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_4d(k_smem + c * 128 * 128, &tma_k, smem_u32(&sh.own_full), c * 64, p.h,
-                    p.kt * 128, p.b);
-        tma_load_4d(v_smem + c * 128 * 128, &tma_v, smem_u32(&sh.own_full), c * 64, p.h,
-                    p.kt * 128, p.b);
-      }
-      ++own;
-      for (int j = 0; j < p.n; ++j) {
-        if (!mbar_wait(smem_u32(&sh.in_empty[pos.slot]), pos.parity ^ 1u, abort_flag, err,
-                       kErrWaitProducer)) {
-          ok = false;
-          break;
-        }
-        const uint32_t bar = smem_u32(&sh.in_full[pos.slot]);
-        const uint32_t dst = ring + pos.slot * STAGE;
-        const int tile = p.first + j;
-        mbar_arrive_expect_tx(bar, 2 * rows_bytes + 1024u);
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_5d(dst + c * 128 * 128, &tma_q, bar, c * 64, 0, p.h, tile * g.tpt, p.b);
-          tma_load_5d(dst + TILE + c * 128 * 128, &tma_do, bar, c * 64, 0, p.h, tile * g.tpt,
-                      p.b);
-        }
-        bulk_load(dst + 2 * TILE, grad_stats(args, p.b, p.h, tile), 1024u, bar);
-        ++issued;
-        pos.step();
-      }
-    }
-    if (!ok) {
-      if (own > 0) mbar_wait_drain(smem_u32(&sh.own_full), (own - 1) & 1u, err);
-      for (int j = max(0, issued - kGradStages); j < issued; ++j)
-        mbar_wait_drain(smem_u32(&sh.in_full[j % kGradStages]), (j / kGradStages) & 1u, err);
-    }
-  } else if (warp == 1 && lane == 0) {
-    // ------------------------------------------------------ MMA issuer
-    // S(j+1) follows dV(j), which reads P(j) in the same columns, and
-    // dP(j+1) follows dK(j) in the same way: MMAs run in issue order.
-    auto wait = [&](const uint64_t* bar, uint32_t parity) {
-      const uint32_t b = smem_u32(bar);
-      return mbar_test_wait(b, parity) || mbar_wait(b, parity, abort_flag, err, kErrWaitMma);
-    };
-    const uint32_t k_lo = smem_desc_lo(k_smem, 16), v_lo = smem_desc_lo(v_smem, 16);
-    bool ok = true;
-    GradRing pos;
-    uint32_t own = 0, cnt = 0;  // items, query tiles so far
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const KvPiece p = kv_piece(args, item);
-      if (p.n == 0) continue;
-      ok = wait(&sh.own_full, own & 1u) && wait(&sh.in_full[pos.slot], pos.parity);
-      if (!ok) break;
-      {
-        const uint32_t q = ring + pos.slot * STAGE;
-        mma_rows<D>(tmem + S_COL, k_lo, smem_desc_lo(q, 16), IDESC_S);
-        mma_commit(smem_u32(&sh.s_full[0]));
-        mma_rows<D>(tmem + DP_COL, v_lo, smem_desc_lo(q + TILE, 16), IDESC_S);
-        mma_commit(smem_u32(&sh.dp_full));
-      }
-      // the previous item's sums have been read out of TMEM
-      if (own > 0) ok = wait(&sh.acc_free, (own - 1) & 1u);
-      for (int j = 0; j < p.n && ok; ++j, ++cnt) {
-        const uint32_t q = ring + pos.slot * STAGE;
-        GradRing nxt = pos;
-        nxt.step();
-        const uint32_t qn = ring + nxt.slot * STAGE;
-        ok = wait(&sh.p_ready, cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        mma_cols(tmem + DV_COL, tmem + S_COL, smem_desc_lo(q + TILE, 128 * 128), IDESC_O, j == 0);
-        if (j + 1 < p.n) {
-          ok = wait(&sh.in_full[nxt.slot], nxt.parity);
-          if (!ok) break;
-          mma_rows<D>(tmem + S_COL, k_lo, smem_desc_lo(qn, 16), IDESC_S);
-          mma_commit(smem_u32(&sh.s_full[0]));
-        }
-        ok = wait(&sh.ds_ready, cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        mma_cols(tmem + DK_COL, tmem + DP_COL, smem_desc_lo(q, 128 * 128), IDESC_O, j == 0);
-        mma_commit(smem_u32(&sh.in_empty[pos.slot]));
-        if (j + 1 < p.n) {
-          mma_rows<D>(tmem + DP_COL, v_lo, smem_desc_lo(qn + TILE, 16), IDESC_S);
-          mma_commit(smem_u32(&sh.dp_full));
-        } else {
-          mma_commit(smem_u32(&sh.acc_full));
-          mma_commit(smem_u32(&sh.own_empty));
-        }
-        pos = nxt;
-      }
-      ++own;
-    }
-    if (!ok) {
-      mma_commit(smem_u32(&sh.drain));
-      mbar_wait_drain(smem_u32(&sh.drain), 0, err);
-    }
+  if (warp == 0) {
+    if (elect_one()) grad_producer<D, 0>(args, sh, maps, base);
+  } else if (warp == 3) {
+    if (elect_one()) grad_producer<D, 1>(args, sh, maps, base);
+  } else if (warp == 1) {
+    if (elect_one()) grad_mma<FMT, D>(args, sh, base, tmem);
   } else if (warp >= 4) {
-    // ------------------------- elementwise: thread = key, 64 packed rows
-    const int wg = (warp - 4) >> 2, q = warp & 3;
-    const int row = q * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t s_t = tmem + lane_addr + S_COL + wg * 64;
-    const uint32_t dp_t = tmem + lane_addr + DP_COL + wg * 64;
-    const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
-    const int off = g.kv_len - g.q_len;
-    bool ok = true;
-    GradRing pos;
-    uint32_t own = 0, cnt = 0;
-    auto wait = [&](const uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu,
-                        mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitSoftmax));
-    };
-    auto release = [&](uint64_t* bar) {
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(bar));
-    };
-    for (int item = blockIdx.x; item < args.items && ok; item += gridDim.x) {
-      const KvPiece p = kv_piece(args, item);
-      const int k0 = p.kt * 128, key = k0 + row;
-      // tokens that see this key: [key - off, key - off + window), or all
-      // later ones for a sink key
-      const int tok_lo = key - off;
-      const int tok_hi = (g.window == kOpsNoWindow || key < g.sinks) ? kOpsMaxLen
-                                                                      : tok_lo + g.window - 1;
-      for (int j = 0; j < p.n; ++j, ++cnt) {
-        const int ta = (p.first + j) * g.tpt, tb = ta + g.tpt - 1;
-        // some key of the tile misses some token of the query tile
-        const bool masked = k0 + 127 - off > ta ||
-                            (g.window != kOpsNoWindow && k0 - off + g.window - 1 < tb);
-        // packed rows of this thread's half that see the key: [c_lo, c_hi)
-        const int c_lo = (max(tok_lo, ta) - ta) * g.g - wg * 64;
-        const int c_hi = (min(tok_hi, tb) - ta + 1) * g.g - wg * 64;
-        // statistics are written by the bulk copy that in_full counts
-        ok = wait(&sh.in_full[pos.slot], pos.parity) && wait(&sh.s_full[0], cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t st = ring + pos.slot * STAGE + 2 * TILE + wg * 256;
-        float pr[64];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          tmem_ld32(s_t + c * 32, *reinterpret_cast<uint32_t(*)[32]>(
-                                      reinterpret_cast<uint32_t*>(pr) + c * 32));
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          float4 nl;
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(nl.x), "=f"(nl.y), "=f"(nl.z), "=f"(nl.w)
-                       : "r"(st + i * 4));
-          const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2,
-                                      make_float2(nl.x, nl.y));
-          const float2 y = __ffma2_rn(make_float2(pr[i + 2], pr[i + 3]), scale2,
-                                      make_float2(nl.z, nl.w));
-          pr[i] = ex2_approx(x.x);
-          pr[i + 1] = ex2_approx(x.y);
-          pr[i + 2] = ex2_approx(y.x);
-          pr[i + 3] = ex2_approx(y.y);
-        }
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t see = bits_below(c_hi, c) & ~bits_below(c_lo, c);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) pr[c * 32 + i] = (see & (1u << i)) ? pr[c * 32 + i] : 0.f;
-          }
-        }
-        {
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk[i] = pack2<FMT>(pr[2 * i], pr[2 * i + 1]);
-          tmem_st32(s_t, pk);
-        }
-        release(&sh.p_ready);
-        ok = wait(&sh.dp_full, cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32];
-          tmem_ld32(dp_t + c * 32, dp);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 dl;
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(dl.x), "=f"(dl.y), "=f"(dl.z), "=f"(dl.w)
-                         : "r"(st + 512 + (c * 32 + i) * 4));
-            const float d[4] = {dl.x, dl.y, dl.z, dl.w};
-            float ds[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float pv = pr[c * 32 + i + u];
-              ds[u] = pv * (__uint_as_float(dp[i + u]) - d[u]);
-            }
-            pk[c * 16 + i / 2] = pack2<FMT>(ds[0], ds[1]);
-            pk[c * 16 + i / 2 + 1] = pack2<FMT>(ds[2], ds[3]);
-          }
-        }
-        if (masked) {
-          // 0 * (dP - delta) is not 0 when the masked dP is not finite
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint32_t see = (bits_below(c_hi, i / 16) & ~bits_below(c_lo, i / 16)) >>
-                                 (2 * (i % 16));
-            pk[i] &= ((see & 1u) ? 0x0000ffffu : 0u) | ((see & 2u) ? 0xffff0000u : 0u);
-          }
-        }
-        tmem_st32(dp_t, pk);
-        release(&sh.ds_ready);
-        pos.step();
-      }
-      if (!ok) break;
-      if (p.n > 0) {
-        ok = wait(&sh.acc_full, own & 1u);
-        if (!ok) break;
-        tc_fence_after();
-      }
-      // warpgroup 0 writes dV, warpgroup 1 dK
-      const uint32_t acc = tmem + lane_addr + (wg == 0 ? DV_COL : DK_COL);
-      const float f = wg == 0 ? 1.f : args.scale;
-      const bool sink = key < g.sinks;
-      T* dst = wg == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
-                             p.h * args.dv_head
-                       : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
-                             p.h * args.dk_head;
-      if (k0 < g.sinks) {
-        float* part = sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + wg * D : nullptr;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(acc + c * 32, r);
-          tmem_wait_ld();
-          if (sink && key < g.kv_len) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + c * 32 + i) =
-                  p.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f,
-                                         __uint_as_float(r[i + 2]) * f,
-                                         __uint_as_float(r[i + 3]) * f);
-          }
-        }
-      }
-      if (p.piece == 0)
-        store_row<T, FMT, D>(acc, dst, f, key < g.kv_len && !sink, p.n == 0);
-      if (p.n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.acc_free));
-        ++own;
-      }
+    const int q = warp & 3;
+    GradEw<T, FMT, D> ew{args, sh, base, tmem, (warp - 4) >> 2, q * 32 + lane, lane,
+                         static_cast<uint32_t>(q * 32) << 16};
+    for (int it = 0; ew.ok; ++it) {
+      int item;
+      if (!grad_next_item<true>(sh, it, &sh.abort, args.err, kErrWaitSoftmax, item) || item < 0)
+        break;
+      if (item < args.kv_items)
+        ew.keys(item);
+      else
+        ew.rows(item);
     }
   }
   tc_fence_before();
@@ -577,264 +898,12 @@ __global__ void __launch_bounds__(2 * D) attn_grad_join_kernel(const GradArgs a)
   *dst = Elem<T>::from_f(s);
 }
 
-// ---------------------------------------------------------------------- dQ
-template <typename T, int FMT, int D>
-__global__ void __launch_bounds__(kGradThreads, 1)
-    attn_grad_q_kernel(const __grid_constant__ CUtensorMap tma_q,
-                       const __grid_constant__ CUtensorMap tma_do,
-                       const __grid_constant__ CUtensorMap tma_k,
-                       const __grid_constant__ CUtensorMap tma_v,
-                       const __grid_constant__ GradArgs args) {
-  constexpr uint32_t TILE = 128u * D * 2;
-  constexpr uint32_t STAGE = 2 * TILE;  // K, V
-  constexpr uint32_t IDESC_S = make_idesc(FMT, 128, 128, false, false);
-  constexpr uint32_t IDESC_O = make_idesc(FMT, 128, D, false, true);
-  // two S buffers (dS overlays S), dP, dQ
-  constexpr uint32_t S_COL = 0, DP_COL = 256, DQ_COL = 384;
-
-  __shared__ GradShared sh;
-  extern __shared__ uint8_t dyn_smem[];
-  const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
-  const uint32_t q_smem = base, do_smem = base + TILE, ring = base + 2 * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const AttnGeom& g = args.geom;
-  unsigned int* err = args.err;
-  const AttnSeq seq{g.q_len, g.kv_len, 0, g.kv_len - g.q_len};
-
-  if (threadIdx.x == 0) {
-    grad_init(sh);
-    tma_prefetch_desc(&tma_q);
-    tma_prefetch_desc(&tma_do);
-    tma_prefetch_desc(&tma_k);
-    tma_prefetch_desc(&tma_v);
-  }
-  if (warp == 2) {
-    tmem_alloc(smem_u32(&sh.tmem_base), 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem_base;
-  volatile int* abort_flag = &sh.abort;
-
-  struct Item {
-    int b, h, t0, t1, tile;
-    AttnBlocks blk;
-  };
-  auto item_of = [&](int item) {
-    Item it;
-    it.h = item % g.heads_kv;
-    const int r = item / g.heads_kv;
-    it.b = r % g.batch;
-    it.tile = g.tiles - 1 - r / g.batch;  // the longest rows first
-    it.t0 = it.tile * g.tpt;
-    it.t1 = min(it.t0 + g.tpt, g.q_len);
-    it.blk = attn_blocks(g, seq, it.t0, it.t1);
-    return it;
-  };
-  const int items = g.tiles * g.batch * g.heads_kv;
-
-  if (warp == 0 && lane == 0) {
-    const uint32_t rows_bytes = static_cast<uint32_t>(g.tpt * g.g) * D * 2;
-    bool ok = true;
-    int issued = 0, own = 0;
-    GradRing pos;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item it = item_of(item);
-      if (it.blk.n == 0) continue;
-      ok = own == 0 || mbar_wait(smem_u32(&sh.own_empty), (own - 1) & 1u, abort_flag, err,
-                                 kErrWaitProducer);
-      if (!ok) break;
-      mbar_arrive_expect_tx(smem_u32(&sh.own_full), 2 * rows_bytes);
-      for (int c = 0; c < D / 64; ++c) {
-        tma_load_5d(q_smem + c * 128 * 128, &tma_q, smem_u32(&sh.own_full), c * 64, 0, it.h,
-                    it.t0, it.b);
-        tma_load_5d(do_smem + c * 128 * 128, &tma_do, smem_u32(&sh.own_full), c * 64, 0, it.h,
-                    it.t0, it.b);
-      }
-      ++own;
-      for (int j = 0; j < it.blk.n; ++j) {
-        if (!mbar_wait(smem_u32(&sh.in_empty[pos.slot]), pos.parity ^ 1u, abort_flag, err,
-                       kErrWaitProducer)) {
-          ok = false;
-          break;
-        }
-        const uint32_t bar = smem_u32(&sh.in_full[pos.slot]);
-        const uint32_t dst = ring + pos.slot * STAGE;
-        mbar_arrive_expect_tx(bar, STAGE);
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(dst + c * 128 * 128, &tma_k, bar, c * 64, it.h, it.blk.at(j) * 128, it.b);
-          tma_load_4d(dst + TILE + c * 128 * 128, &tma_v, bar, c * 64, it.h, it.blk.at(j) * 128,
-                      it.b);
-        }
-        ++issued;
-        pos.step();
-      }
-    }
-    if (!ok) {
-      if (own > 0) mbar_wait_drain(smem_u32(&sh.own_full), (own - 1) & 1u, err);
-      for (int j = max(0, issued - kGradStages); j < issued; ++j)
-        mbar_wait_drain(smem_u32(&sh.in_full[j % kGradStages]), (j / kGradStages) & 1u, err);
-    }
-  } else if (warp == 1 && lane == 0) {
-    // S(j+1) goes to the other buffer before dS(j) is waited for; dP(j+1)
-    // then has its columns back (they are read by the time dS(j) is ready)
-    // and comes before dQ(j), so that the elementwise warps wait least.
-    auto wait = [&](const uint64_t* bar, uint32_t parity) {
-      const uint32_t b = smem_u32(bar);
-      return mbar_test_wait(b, parity) || mbar_wait(b, parity, abort_flag, err, kErrWaitMma);
-    };
-    const uint32_t q_lo = smem_desc_lo(q_smem, 16), do_lo = smem_desc_lo(do_smem, 16);
-    bool ok = true;
-    GradRing pos;
-    uint32_t own = 0, cnt = 0;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item it = item_of(item);
-      const int n = it.blk.n;
-      if (n == 0) continue;
-      ok = wait(&sh.own_full, own & 1u) && wait(&sh.in_full[pos.slot], pos.parity);
-      if (!ok) break;
-      {
-        const uint32_t k = ring + pos.slot * STAGE;
-        mma_rows<D>(tmem + S_COL + (cnt & 1u) * 128, q_lo, smem_desc_lo(k, 16), IDESC_S);
-        mma_commit(smem_u32(&sh.s_full[cnt & 1u]));
-        mma_rows<D>(tmem + DP_COL, do_lo, smem_desc_lo(k + TILE, 16), IDESC_S);
-        mma_commit(smem_u32(&sh.dp_full));
-      }
-      if (own > 0) ok = wait(&sh.acc_free, (own - 1) & 1u);
-      for (int j = 0; j < n && ok; ++j, ++cnt) {
-        const uint32_t k = ring + pos.slot * STAGE;
-        GradRing nxt = pos;
-        nxt.step();
-        const uint32_t kn = ring + nxt.slot * STAGE;
-        if (j + 1 < n) {
-          ok = wait(&sh.in_full[nxt.slot], nxt.parity);
-          if (!ok) break;
-          mma_rows<D>(tmem + S_COL + ((cnt + 1) & 1u) * 128, q_lo, smem_desc_lo(kn, 16), IDESC_S);
-          mma_commit(smem_u32(&sh.s_full[(cnt + 1) & 1u]));
-        }
-        ok = wait(&sh.ds_ready, cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        if (j + 1 < n) {
-          mma_rows<D>(tmem + DP_COL, do_lo, smem_desc_lo(kn + TILE, 16), IDESC_S);
-          mma_commit(smem_u32(&sh.dp_full));
-        } else {
-          mma_commit(smem_u32(&sh.own_empty));
-        }
-        mma_cols(tmem + DQ_COL, tmem + S_COL + (cnt & 1u) * 128, smem_desc_lo(k, 128 * 128),
-                 IDESC_O, j == 0);
-        mma_commit(smem_u32(&sh.in_empty[pos.slot]));
-        if (j + 1 == n) mma_commit(smem_u32(&sh.acc_full));
-        pos = nxt;
-      }
-      ++own;
-    }
-    if (!ok) {
-      mma_commit(smem_u32(&sh.drain));
-      mbar_wait_drain(smem_u32(&sh.drain), 0, err);
-    }
-  } else if (warp >= 4) {
-    // --------------------- elementwise: thread = packed row, 64 keys
-    const int wg = (warp - 4) >> 2, q = warp & 3;
-    const int row = q * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t dp_t = tmem + lane_addr + DP_COL + wg * 64;
-    const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
-    const int row_token = row / g.g, row_head = row % g.g;
-    bool ok = true;
-    uint32_t own = 0, cnt = 0;
-    auto wait = [&](const uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu,
-                        mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitSoftmax));
-    };
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const Item it = item_of(item);
-      const int token = it.t0 + row_token;
-      const bool live = row_token < g.tpt && token < it.t1;
-      const float* st = grad_stats(args, it.b, it.h, it.tile);
-      const float nl = st[row], delta = st[128 + row];
-      const float2 shift2 = make_float2(nl, nl);
-      for (int j = 0; j < it.blk.n; ++j, ++cnt) {
-        const int key0 = it.blk.at(j) * 128;
-        const bool masked = block_is_masked(g, seq, it.t0, it.t1, key0);
-        const RowMask rm = row_mask(g, token + seq.off, key0 + wg * 64);
-        const uint32_t s_t = tmem + lane_addr + S_COL + (cnt & 1u) * 128 + wg * 64;
-        ok = wait(&sh.s_full[cnt & 1u], (cnt >> 1) & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        float pr[64];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          tmem_ld32(s_t + c * 32, *reinterpret_cast<uint32_t(*)[32]>(
-                                      reinterpret_cast<uint32_t*>(pr) + c * 32));
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2, shift2);
-          pr[i] = ex2_approx(x.x);
-          pr[i + 1] = ex2_approx(x.y);
-        }
-        ok = wait(&sh.dp_full, cnt & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t dp[32];
-          tmem_ld32(dp_t + c * 32, dp);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            pk[c * 16 + i / 2] =
-                pack2<FMT>(pr[c * 32 + i] * (__uint_as_float(dp[i]) - delta),
-                           pr[c * 32 + i + 1] * (__uint_as_float(dp[i + 1]) - delta));
-          if (masked) {
-            const uint32_t see = rm.word(c);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              pk[c * 16 + i] &= ((see & (1u << (2 * i))) ? 0x0000ffffu : 0u) |
-                                ((see & (2u << (2 * i))) ? 0xffff0000u : 0u);
-          }
-        }
-        tmem_st32(s_t, pk);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_ready));
-      }
-      if (!ok) break;
-      if (it.blk.n > 0) {
-        ok = wait(&sh.acc_full, own & 1u);
-        if (!ok) break;
-        tc_fence_after();
-      }
-      // each warpgroup writes half of the dims
-      T* dst = static_cast<T*>(args.dq) + it.b * args.dq_batch + token * args.dq_token +
-               (it.h * g.g + row_head) * args.dq_head + wg * (D / 2);
-      store_row<T, FMT, D / 2>(tmem + lane_addr + DQ_COL + wg * (D / 2), dst, args.scale, live,
-                               it.blk.n == 0);
-      if (it.blk.n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.acc_free));
-        ++own;
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (warp == 2) tmem_dealloc(tmem, 512);
-}
-
 // ------------------------------------------------------------------- host
 namespace {
 
 struct GradPlan {
   int kv_tiles, sink_tiles, far_tiles, far_pieces;
-  uint64_t stats_bytes, partial_bytes;
+  uint64_t stats_bytes, partial_bytes;  // behind 256 bytes for the item counter
 };
 
 GradPlan grad_plan(const AttnGeom& g, int dim) {
@@ -869,8 +938,10 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   const GradPlan pl = grad_plan(g, D);
   GradArgs a{};
   a.geom = g;
-  a.stats = static_cast<float*>(gp.workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<char*>(gp.workspace) + pl.stats_bytes);
+  char* work = static_cast<char*>(gp.workspace);
+  a.next = reinterpret_cast<unsigned int*>(work);
+  a.stats = reinterpret_cast<float*>(work + 256);
+  a.partial = reinterpret_cast<float*>(work + 256 + pl.stats_bytes);
   a.out = gp.out.ptr;
   a.dout = gp.dout.ptr;
   a.lse = gp.lse;
@@ -898,36 +969,24 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   const int64_t q_items = heads * g.tiles;
   const int64_t kv_items = heads * (pl.kv_tiles + static_cast<int64_t>(pl.sink_tiles) * pl.far_pieces);
   const int64_t most = (1ll << 31) - 1024;
-  if (q_items > most || kv_items > most || heads * g.sinks > most) return GPO_BAD_ARGS;
-  a.items = static_cast<int>(kv_items);
+  if (q_items + kv_items > most || heads * g.sinks > most) return GPO_BAD_ARGS;
+  a.kv_items = static_cast<int>(kv_items);
+  a.items = static_cast<int>(q_items + kv_items);
+  if (a.items == 0) return GPO_OK;
   const int sms = c.sm_count > 0 ? c.sm_count : 148;
-  if (q_items > 0) {
-    attn_grad_stats_kernel<T, D><<<static_cast<unsigned>(q_items), 256, 0, c.stream>>>(a);
-    if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
-  }
-  constexpr uint32_t tile = 128u * D * 2u;
-  if (kv_items > 0) {
-    constexpr uint32_t dyn = 2 * tile + kGradStages * (2 * tile + 1024u) + 1024u;
-    auto kern = attn_grad_kv_kernel<T, FMT, D>;
-    const gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
-    if (s != GPO_OK) return s;
-    kern<<<static_cast<unsigned>(std::min<int64_t>(kv_items, sms)), kGradThreads, dyn,
-           c.stream>>>(mq, mdo, mk, mv, a);
-    if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
-    if (pl.sink_tiles > 0) {
-      attn_grad_join_kernel<T, D>
-          <<<static_cast<unsigned>(heads * g.sinks), 2 * D, 0, c.stream>>>(a);
-      if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
-    }
-  }
-  if (q_items > 0) {
-    constexpr uint32_t dyn = 2 * tile + kGradStages * 2 * tile + 1024u;
-    auto kern = attn_grad_q_kernel<T, FMT, D>;
-    const gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
-    if (s != GPO_OK) return s;
-    kern<<<static_cast<unsigned>(std::min<int64_t>(q_items, sms)), kGradThreads, dyn,
-           c.stream>>>(mq, mdo, mk, mv, a);
-  }
+  attn_grad_stats_kernel<T, D>
+      <<<static_cast<unsigned>(std::max<int64_t>(1, q_items)), 256, 0, c.stream>>>(a);
+  if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
+  auto kern = attn_grad_kernel<T, FMT, D>;
+  constexpr uint32_t dyn = GradGeom<D>::BYTES;
+  const gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
+  if (s != GPO_OK) return s;
+  kern<<<static_cast<unsigned>(std::min(a.items, sms)), kGradThreads, dyn, c.stream>>>(mq, mdo, mk,
+                                                                                      mv, a);
+  if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
+  if (pl.sink_tiles > 0)
+    attn_grad_join_kernel<T, D>
+        <<<static_cast<unsigned>(heads * g.sinks), 2 * D, 0, c.stream>>>(a);
   return launch_status();
 }
 
@@ -935,7 +994,7 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
 
 uint64_t attn_grad_workspace(const AttnProblem& p) {
   const GradPlan pl = grad_plan(p.geom, p.dim);
-  return pl.stats_bytes + pl.partial_bytes;
+  return 256u + pl.stats_bytes + pl.partial_bytes;
 }
 
 gpo_status launch_attn_grad(const AttnProblem& p, const AttnGradProblem& gp, const LaunchCtx& c) {
