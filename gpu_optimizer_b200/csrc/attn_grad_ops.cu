@@ -36,11 +36,12 @@ namespace gpo {
 constexpr int kGradA = 3, kGradB = 2;  // ring depths
 constexpr int kGradThreads = 384;      // 4 service warps, 2 x 4 elementwise warps
 constexpr int kGradEwWarps = 8;
+constexpr int kGradFma = 2;             // of 4 pairs of exponentials (see exp2_to)
 constexpr int kGradReaders = 2 + kGradEwWarps;  // of an item: warp 3, warp 1, elementwise
 
 struct GradArgs {
   AttnGeom geom;
-  // per packed row: -L in the log2 domain, and delta; 128 + 128 floats per
+  // per packed row: -L in the log2 domain, and -delta; 128 + 128 floats per
   // (batch, kv head, query tile)
   float* stats;
   // sums of dK and dV rows of sink keys that several CTAs share
@@ -57,6 +58,7 @@ struct GradArgs {
   int far_pieces;  // far pieces of a sink tile
   int kv_items, items;     // items [0, kv_items): key tiles, then query tiles
   unsigned int* next;      // counter of items, zeroed by the statistics kernel
+  bool wide_dq, wide_dkv;  // rows on 32 bytes
   unsigned int* err;
 };
 
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
         nl = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
       }
       st[r] = nl;
-      st[128 + r] = live ? s : 0.f;
+      st[128 + r] = live ? -s : 0.f;
     }
   }
 }
@@ -120,7 +122,7 @@ struct GradShared {
   uint64_t s_full[2], dp_full;       // key tiles use s_full[0] alone
   uint64_t q_s_full[2];              // the two S buffers of query tiles
   uint64_t p_ready, ds_ready;
-  uint64_t acc_full, acc_free;
+  uint64_t dv_full, acc_full, acc_free;
   uint64_t item_full[2], item_empty[2];
   uint64_t drain;
   int item[2];
@@ -157,6 +159,7 @@ __device__ __forceinline__ void grad_init(GradShared& sh) {
   init(sh.q_s_full, 2, 1);
   init(&sh.p_ready, 1, kGradEwWarps);
   init(&sh.ds_ready, 1, kGradEwWarps);
+  init(&sh.dv_full, 1, 1);
   init(&sh.acc_full, 1, 1);
   init(&sh.acc_free, 1, kGradEwWarps);
   init(sh.item_full, 2, 1);
@@ -221,7 +224,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // One row of N fp32 TMEM columns, times `f`, to N 16-bit elements at dst.
 template <typename T, int FMT, int N>
-__device__ __forceinline__ void store_row(uint32_t taddr, T* dst, float f, bool live, bool zero) {
+__device__ __forceinline__ void store_row(uint32_t taddr, T* dst, float f, bool live, bool zero,
+                                          bool wide) {
 #pragma unroll
   for (int c = 0; c < N / 32; ++c) {
     uint32_t r[32];
@@ -233,10 +237,8 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, float f, bool 
     for (int i = 0; i < 16; ++i)
       pk[i] = zero ? 0u : pack2<FMT>(__uint_as_float(r[2 * i]) * f,
                                      __uint_as_float(r[2 * i + 1]) * f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      reinterpret_cast<uint4*>(dst + c * 32)[i] =
-          make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+    store_pairs8(dst + c * 32, pk, wide);
+    store_pairs8(dst + c * 32 + 16, pk + 8, wide);
   }
 }
 
@@ -496,6 +498,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
         tc_fence_after();
         mma_cols(tmem + C::DV, tmem + C::S, cols_of(G::RING_B, bj), IDESC_O, j == 0);
         commit(&sh.b_empty[bj]);
+        if (!more) commit(&sh.dv_full);
         a.step();
         b.step();
         if (more) {
@@ -586,7 +589,7 @@ struct GradEw {
   uint32_t lane_addr;
   bool ok = true;
   GradRing<2> st;
-  uint32_t own = 0, cnt = 0, qcnt = 0;
+  uint32_t own = 0, kown = 0, cnt = 0, qcnt = 0;  // items, key tiles; steps, of query tiles
 
   __device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity) {
     return ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &sh.abort, args.err,
@@ -605,6 +608,25 @@ struct GradEw {
       tmem_ld32(taddr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(
                                     reinterpret_cast<uint32_t*>(x) + c * 32));
     tmem_wait_ld();
+  }
+  // P of a pair.  The exponentials take the special function unit 1024
+  // cycles per step (16 a cycle), longer than anything else the elementwise
+  // warps do, so kGradFma of every 4 pairs run on the FMA pipe.
+  static __device__ __forceinline__ void exp2_to(float (&pr)[64], int i, float2 x) {
+    float2 y;
+    if ((i / 2) % 4 < kGradFma)
+      y = exp2_fma<FMT == 1 ? 3 : 4>(x);
+    else
+      y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    pr[i] = y.x;
+    pr[i + 1] = y.y;
+  }
+  // dS = P * (dP - delta) of a pair
+  static __device__ __forceinline__ uint32_t ds_pair(const float (&pr)[64], int i,
+                                                     const uint32_t (&dp)[32], int k, float2 nd) {
+    const float2 d = __fadd2_rn(make_float2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), nd);
+    const float2 s = __fmul2_rn(make_float2(pr[i], pr[i + 1]), d);
+    return pack2<FMT>(s.x, s.y);
   }
   __device__ __forceinline__ void acc_release() {
     tc_fence_before();
@@ -648,14 +670,10 @@ struct GradEw {
         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(nl.x), "=f"(nl.y), "=f"(nl.z), "=f"(nl.w)
                      : "r"(stat + i * 4));
-        const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2,
-                                    make_float2(nl.x, nl.y));
-        const float2 y = __ffma2_rn(make_float2(pr[i + 2], pr[i + 3]), scale2,
-                                    make_float2(nl.z, nl.w));
-        pr[i] = ex2_approx(x.x);
-        pr[i + 1] = ex2_approx(x.y);
-        pr[i + 2] = ex2_approx(y.x);
-        pr[i + 3] = ex2_approx(y.y);
+        exp2_to(pr, i, __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2,
+                                  make_float2(nl.x, nl.y)));
+        exp2_to(pr, i + 2, __ffma2_rn(make_float2(pr[i + 2], pr[i + 3]), scale2,
+                                      make_float2(nl.z, nl.w)));
       }
       if (masked) {
 #pragma unroll
@@ -686,13 +704,8 @@ struct GradEw {
           asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                        : "=f"(dl.x), "=f"(dl.y), "=f"(dl.z), "=f"(dl.w)
                        : "r"(stat + 512 + (c * 32 + i) * 4));
-          const float d[4] = {dl.x, dl.y, dl.z, dl.w};
-          float ds[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            ds[u] = pr[c * 32 + i + u] * (__uint_as_float(dp[i + u]) - d[u]);
-          pk[c * 16 + i / 2] = pack2<FMT>(ds[0], ds[1]);
-          pk[c * 16 + i / 2 + 1] = pack2<FMT>(ds[2], ds[3]);
+          pk[c * 16 + i / 2] = ds_pair(pr, c * 32 + i, dp, i, make_float2(dl.x, dl.y));
+          pk[c * 16 + i / 2 + 1] = ds_pair(pr, c * 32 + i + 2, dp, i + 2, make_float2(dl.z, dl.w));
         }
       }
       if (masked) {
@@ -709,37 +722,46 @@ struct GradEw {
       if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
       st.step();
     }
-    if (p.n > 0) {
-      if (!wait(&sh.acc_full, own & 1u)) return;
-      tc_fence_after();
-    }
-    // warpgroup 0 writes dV, warpgroup 1 dK
-    const uint32_t acc = tmem + lane_addr + (wg == 0 ? C::DV : C::DK);
-    const float f = wg == 0 ? 1.f : args.scale;
-    const bool sink = key < g.sinks;
-    T* dst = wg == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
-                           p.h * args.dv_head
-                     : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
-                           p.h * args.dk_head;
-    if (k0 < g.sinks) {
-      float* part = sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + wg * D : nullptr;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(acc + c * 32, r);
-        tmem_wait_ld();
-        if (sink && key < g.kv_len) {
+    // dV first, while the last dK product still runs; each warpgroup has
+    // half of the dims
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(part + c * 32 + i) =
-                p.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                         : make_float4(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f,
-                                       __uint_as_float(r[i + 2]) * f,
-                                       __uint_as_float(r[i + 3]) * f);
+    for (int m = 0; m < 2; ++m) {
+      if (p.n > 0) {
+        if (!wait(m == 0 ? &sh.dv_full : &sh.acc_full, (m == 0 ? kown : own) & 1u)) return;
+        tc_fence_after();
+      }
+      constexpr int H = D / 2;
+      const uint32_t acc = tmem + lane_addr + (m == 0 ? C::DV : C::DK) + wg * H;
+      const float f = m == 0 ? 1.f : args.scale;
+      const bool sink = key < g.sinks;
+      if (k0 < g.sinks) {
+        float* part =
+            sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + m * D + wg * H : nullptr;
+#pragma unroll 1
+        for (int c = 0; c < H / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(acc + c * 32, r);
+          tmem_wait_ld();
+          if (sink && key < g.kv_len) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + c * 32 + i) =
+                  p.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                           : make_float4(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f,
+                                         __uint_as_float(r[i + 2]) * f,
+                                         __uint_as_float(r[i + 3]) * f);
+          }
         }
       }
+      T* dst = m == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
+                            p.h * args.dv_head
+                      : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
+                            p.h * args.dk_head;
+      if (p.piece == 0)
+        store_row<T, FMT, H>(acc, dst + wg * H, f, key < g.kv_len && !sink, p.n == 0,
+                             args.wide_dkv);
     }
-    if (p.piece == 0) store_row<T, FMT, D>(acc, dst, f, key < g.kv_len && !sink, p.n == 0);
+    if (p.n > 0) ++kown;
     if (p.n > 0) acc_release();
   }
 
@@ -754,8 +776,8 @@ struct GradEw {
     const int token = it.t0 + row_token;
     const bool live = row_token < g.tpt && token < it.t1;
     const float* stat = grad_stats(args, it.b, it.h, it.tile);
-    const float nl = stat[row], delta = stat[128 + row];
-    const float2 shift2 = make_float2(nl, nl);
+    const float nl = stat[row], nd = stat[128 + row];
+    const float2 shift2 = make_float2(nl, nl), delta2 = make_float2(nd, nd);
     for (int j = 0; j < it.blk.n; ++j, ++cnt, ++qcnt) {
       const int key0 = it.blk.at(j) * 128;
       const bool masked = block_is_masked(g, it.seq, it.t0, it.t1, key0);
@@ -767,9 +789,7 @@ struct GradEw {
       load64(s_t, pr);
 #pragma unroll
       for (int i = 0; i < 64; i += 2) {
-        const float2 x = __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2, shift2);
-        pr[i] = ex2_approx(x.x);
-        pr[i + 1] = ex2_approx(x.y);
+        exp2_to(pr, i, __ffma2_rn(make_float2(pr[i], pr[i + 1]), scale2, shift2));
       }
       if (!wait(&sh.dp_full, cnt & 1u)) return;
       tc_fence_after();
@@ -781,8 +801,7 @@ struct GradEw {
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
-          pk[c * 16 + i / 2] = pack2<FMT>(pr[c * 32 + i] * (__uint_as_float(dp[i]) - delta),
-                                          pr[c * 32 + i + 1] * (__uint_as_float(dp[i + 1]) - delta));
+          pk[c * 16 + i / 2] = ds_pair(pr, c * 32 + i, dp, i, delta2);
         if (masked) {
           const uint32_t see = rm.word(c);
 #pragma unroll
@@ -802,7 +821,7 @@ struct GradEw {
     T* dst = static_cast<T*>(args.dq) + it.b * args.dq_batch + token * args.dq_token +
              (it.h * g.g + row_head) * args.dq_head + wg * (D / 2);
     store_row<T, FMT, D / 2>(tmem + lane_addr + C::DQ + wg * (D / 2), dst, args.scale, live,
-                             it.blk.n == 0);
+                             it.blk.n == 0, args.wide_dq);
     if (it.blk.n > 0) acc_release();
   }
 };
@@ -958,6 +977,8 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   strides(gp.dq, a.dq_batch, a.dq_token, a.dq_head);
   strides(gp.dk, a.dk_batch, a.dk_token, a.dk_head);
   strides(gp.dv, a.dv_batch, a.dv_token, a.dv_head);
+  a.wide_dq = rows_on_32(gp.dq);
+  a.wide_dkv = rows_on_32(gp.dk) && rows_on_32(gp.dv);
   a.scale = p.scale;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.kv_tiles = pl.kv_tiles;

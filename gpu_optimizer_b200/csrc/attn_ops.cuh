@@ -117,6 +117,48 @@ __device__ __forceinline__ bool block_is_masked(const AttnGeom& g, const AttnSeq
                                             key0 + kOpsBN > g.sinks);
 }
 
+// 2^x of two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by
+// a polynomial of least relative error on that interval (7.5e-5 of degree 3,
+// 2.6e-6 of degree 4; fitted by iteratively reweighted least squares), n added
+// to the exponent.  For values that are rounded to 16 bits next (degree 3:
+// bfloat16, 4: float16).  x below -126 gives at most 2^-126.
+template <int DEGREE>
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to integer
+  auto both = [](float v) { return make_float2(v, v); };
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 n = __fadd2_rn(x, both(kRound));
+  const float2 f = __fadd2_rn(x, __ffma2_rn(n, both(-1.f), both(kRound)));
+  float2 p;
+  if constexpr (DEGREE == 3) {
+    p = __ffma2_rn(f, both(0.05517167f), both(0.24261113f));
+    p = __ffma2_rn(f, p, both(0.69326097f));
+    p = __ffma2_rn(f, p, both(0.99992806f));
+  } else {
+    p = __ffma2_rn(f, both(0.009570102f), both(0.05591786f));
+    p = __ffma2_rn(f, p, both(0.24024744f));
+    p = __ffma2_rn(f, p, both(0.6931218f));
+    p = __ffma2_rn(f, p, both(0.9999993f));
+  }
+  // the integer n sits in the low bits of n + kRound
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// Eight 16-bit pairs to global memory: one 32-byte store where the address
+// allows (a row per lane: a whole sector per lane and half the wavefronts).
+__device__ __forceinline__ void store_pairs8(void* dst, const uint32_t* v, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
 // True in one thread of a converged warp.  Single-thread roles branch on this
 // and not on the lane index: the compiler then knows that one thread runs
 // and keeps descriptors in uniform registers.  Measured: 38 cycles to issue
@@ -155,6 +197,12 @@ struct HeadsView {
   int64_t batch, tokens, heads;
   int64_t s_batch, s_token, s_head;  // elements
 };
+
+// Whether every row of `t` starts on 32 bytes (see store_pairs8).
+inline bool rows_on_32(const HeadsView& t) {
+  return (reinterpret_cast<uintptr_t>(t.ptr) & 31u) == 0 && (t.batch <= 1 || t.s_batch % 16 == 0) &&
+         (t.tokens <= 1 || t.s_token % 16 == 0) && (t.heads <= 1 || t.s_head % 16 == 0);
+}
 
 // Tile of a query-side tensor: {64 dims, g heads, 1 kv head, tpt tokens}.
 bool encode_rows_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, int g, int tpt);
