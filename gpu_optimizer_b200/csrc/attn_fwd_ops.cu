@@ -72,7 +72,8 @@ struct FwdArgs {
   float scale_log2;
   int spans;     // units of a sequence and kv head (of the longest sequence)
   int items;
-  int stages;
+  int k_stages, v_stages;
+  bool wide;     // rows of out on 32 bytes
   // cut launches
   unsigned int* arrived;  // per unit and tile, 0 between launches
   float* part;            // [CTA][2] parts of part_rows rows: D floats each, then (m, l)
@@ -279,6 +280,54 @@ __device__ __forceinline__ void fwd_barrier(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
+// Joins the parts [c0, c1] of a unit's elements (of which this thread has
+// every 128th), in their order and against a running maximum.  U elements
+// times P parts are loaded before the first is used: the loop is bound by
+// the latency of these loads.
+template <int U, int P, typename Load, typename Finish>
+__device__ __forceinline__ void fwd_join(int first, int total, int rows, int c0, int c1,
+                                         Load&& load, Finish&& finish) {
+  for (int e0 = first; e0 < total; e0 += 128 * U) {
+    float4 o[U];
+    float m[U], sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      m[u] = -INFINITY;
+      sum[u] = 0.f;
+    }
+    for (int c = c0; c <= c1; c += P) {
+      float2 ml[U][P];
+      float4 v[U][P];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = min(e0 + u * 128, total - 1);
+#pragma unroll
+        for (int i = 0; i < P; ++i) load(c + i, e % rows, e / rows, ml[u][i], v[u][i]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+          if (ml[u][i].y != 0.f) {  // a part without a key says nothing
+            const float to = fmaxf(m[u], ml[u][i].x);
+            const float a = ex2_approx(m[u] - to), f = ex2_approx(ml[u][i].x - to);
+            m[u] = to;
+            sum[u] = sum[u] * a + ml[u][i].y * f;
+            o[u].x = o[u].x * a + v[u][i].x * f;
+            o[u].y = o[u].y * a + v[u][i].y * f;
+            o[u].z = o[u].z * a + v[u][i].z * f;
+            o[u].w = o[u].w * a + v[u][i].w * f;
+          }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * 128;
+      if (e < total) finish(e % rows, e / rows, o[u], m[u], sum[u]);
+    }
+  }
+}
+
 template <int D>
 struct FwdGeom {
   static constexpr int SW = 128;  // swizzle atom: 64 dims of a row
@@ -300,6 +349,7 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
   uint64_t* empty = is_k ? sh.k_empty : sh.v_empty;
   volatile int* abort_flag = &sh.abort;
   const int boxes = PAGED ? kOpsBN / g.box_rows : 1;
+  const int stages = is_k ? args.k_stages : args.v_stages;
   bool ok = true;
   int issued = 0, q_loads = 0;
   RingPos2 pos;
@@ -366,14 +416,14 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[pos.slot]));
       }
-      pos.step(args.stages);
+      pos.step(stages);
     }
   }
   if (!ok && lane == 0) {
     // let the copies in flight land before the CTA can exit
     if (q_loads > 0) mbar_wait_drain(smem_u32(&sh.q_full), (q_loads - 1) & 1u, args.err);
-    for (int j = max(0, issued - args.stages); j < issued; ++j)
-      mbar_wait_drain(smem_u32(&full[j % args.stages]), (j / args.stages) & 1u, args.err);
+    for (int j = max(0, issued - stages); j < issued; ++j)
+      mbar_wait_drain(smem_u32(&full[j % stages]), (j / stages) & 1u, args.err);
   }
 }
 
@@ -390,7 +440,6 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
   const AttnGeom& g = args.geom;
   unsigned int* err = args.err;
   volatile int* abort_flag = &sh.abort;
-  const int stages = args.stages;
   // Between two MMA groups this thread does as little as it can: descriptor
   // halves advance by constants, waits test the phase without blocking first.
   auto wait = [&](const uint64_t* bar, uint32_t parity) {
@@ -446,7 +495,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
           s_mma(0, spos.slot, kpos.slot);
           mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
           if (i == n - 1) mma_commit(smem_u32(&sh.q_empty));
-          kpos.step(stages);
+          kpos.step(args.k_stages);
           spos.step(NB);
         }
         const int j = i - LAG;
@@ -462,7 +511,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
           mma_commit(smem_u32(&sh.pv_done[ppos.slot]));
           mma_commit(smem_u32(&sh.v_empty[vpos.slot]));
           if (j == n - 1) mma_commit(smem_u32(&sh.o_full[0]));
-          vpos.step(stages);
+          vpos.step(args.v_stages);
           ppos.step(NB);
         }
       }
@@ -488,7 +537,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
         if (now[t]) s_mma(t, t, kpos.slot);
       }
       mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
-      kpos.step(stages);
+      kpos.step(args.k_stages);
       if (s.i1 - s.i0 == 1) mma_commit(smem_u32(&sh.q_empty));
       for (int i = s.i0; i < s.i1; ++i) {
         const bool more = i + 1 < s.i1;
@@ -549,10 +598,10 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
         if (more) {
           mma_commit(smem_u32(&sh.k_empty[kpos.slot]));
           if (i + 2 == s.i1) mma_commit(smem_u32(&sh.q_empty));
-          kpos.step(stages);
+          kpos.step(args.k_stages);
         }
         mma_commit(smem_u32(&sh.v_empty[vpos.slot]));
-        vpos.step(stages);
+        vpos.step(args.v_stages);
 #pragma unroll
         for (int t = 0; t < 2; ++t) now[t] = then[t];
       }
@@ -567,8 +616,8 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
 
 // ---------------------------------------------------- softmax and epilogue
 template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
-__device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, float2* join_ml,
-                                            uint32_t tmem, int warp, int lane) {
+__device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, uint32_t tmem,
+                                            int warp, int lane) {
   constexpr int BN = kOpsBN;
   constexpr uint32_t S_COL = TILES * D;
   const AttnGeom& g = args.geom;
@@ -740,15 +789,15 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
         T* orow = static_cast<T*>(args.out) + (PAGED ? 0 : s.b * args.o_batch) +
                   r * args.o_token + head * args.o_head;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t pk[4];
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t pk[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lo = __uint_as_float(ov[c * 8 + 2 * e]) * inv_l;
-            const float hi = __uint_as_float(ov[c * 8 + 2 * e + 1]) * inv_l;
+          for (int e = 0; e < 8; ++e) {
+            const float lo = __uint_as_float(ov[c * 16 + 2 * e]) * inv_l;
+            const float hi = __uint_as_float(ov[c * 16 + 2 * e + 1]) * inv_l;
             pk[e] = FMT == 1 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
           }
-          reinterpret_cast<uint4*>(orow)[c] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          store_pairs8(orow + c * 16, pk, args.wide);
         }
       }
       continue;
@@ -796,75 +845,33 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
       const bool join = *reinterpret_cast<volatile int*>(&sh.last[t]) != 0;
       if (join) {
         __threadfence();
-        // maximum and 1 / sum of each row over the parts, in their order
-        if (row < rows) {
-          float m = -INFINITY, sum = 0.f;
-#pragma unroll 4
-          for (int c = c_first; c <= c_last; ++c) {
-            const float2 ml = __ldcg(part_ml(part_of(c)) + base + row);
-            if (ml.y != 0.f) m = fmaxf(m, ml.x);  // a part without a key says nothing
-          }
-#pragma unroll 4
-          for (int c = c_first; c <= c_last; ++c) {
-            const float2 ml = __ldcg(part_ml(part_of(c)) + base + row);
-            if (ml.y != 0.f) sum += ml.y * ex2_approx(ml.x - m);
-          }
-          join_ml[t * 128 + row] = make_float2(m, sum == 0.f ? 0.f : 1.0f / sum);
-          if (args.lse) {
-            const int tok = tile.t0 + row / g.g;
-            args.lse[lse_at(s.seq.row0 + tok, tok, s.h * g.g + row % g.g)] =
+        // An element is four dims of a row.  Few rows come with many parts
+        // (their unit spans many CTAs), many rows with two or three.
+        auto finish = [&](int r, int x, const float4& o, float m, float sum) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          const int tok = tile.t0 + r / g.g, hd = s.h * g.g + r % g.g;
+          const int64_t at = s.seq.row0 + tok;
+          if (args.lse && x == 0)
+            args.lse[lse_at(at, tok, hd)] =
                 sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
-          }
-        }
-        fwd_barrier(1 + t);
-        // kJoin elements (four dims of a row) per thread at a time, whose
-        // loads are all in flight at once
-        constexpr int kJoin = 4;
+          T* orow = static_cast<T*>(args.out) + at * args.o_token + hd * args.o_head;
+          const uint32_t lo = FMT == 1 ? pack_bf16(o.x * inv, o.y * inv)
+                                       : pack_f16(o.x * inv, o.y * inv);
+          const uint32_t hi = FMT == 1 ? pack_bf16(o.z * inv, o.w * inv)
+                                       : pack_f16(o.z * inv, o.w * inv);
+          reinterpret_cast<uint2*>(orow)[x] = make_uint2(lo, hi);
+        };
+        auto part_row = [&](int c, int r, int x, float2& ml, float4& v) {
+          float* part = part_of(min(c, c_last));
+          ml = __ldcg(part_ml(part) + base + r);
+          v = __ldcg(reinterpret_cast<const float4*>(part) + base + r + x * args.part_rows);
+          if (c > c_last) ml.y = 0.f;
+        };
         const int total = rows * (D / 4);
-        for (int e0 = row; e0 < total; e0 += 128 * kJoin) {
-          float4 o[kJoin];
-          int r[kJoin], x[kJoin];
-          float m[kJoin];
-#pragma unroll
-          for (int u = 0; u < kJoin; ++u) {
-            const int e = e0 + u * 128;
-            r[u] = e < total ? e % rows : -1;
-            x[u] = e / rows;
-            m[u] = r[u] >= 0 ? join_ml[t * 128 + r[u]].x : 0.f;
-            o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll 4
-          for (int c = c_first; c <= c_last; ++c) {
-            float* part = part_of(c);
-#pragma unroll
-            for (int u = 0; u < kJoin; ++u) {
-              if (r[u] < 0) continue;
-              const float2 ml = __ldcg(part_ml(part) + base + r[u]);
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + base + r[u] +
-                                      x[u] * args.part_rows);
-              if (ml.y != 0.f) {
-                const float f = ex2_approx(ml.x - m[u]);
-                o[u].x += v.x * f;
-                o[u].y += v.y * f;
-                o[u].z += v.z * f;
-                o[u].w += v.w * f;
-              }
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < kJoin; ++u) {
-            if (r[u] < 0) continue;
-            const float inv = join_ml[t * 128 + r[u]].y;
-            T* orow = static_cast<T*>(args.out) +
-                      (s.seq.row0 + tile.t0 + r[u] / g.g) * args.o_token +
-                      (s.h * g.g + r[u] % g.g) * args.o_head;
-            const uint32_t lo = FMT == 1 ? pack_bf16(o[u].x * inv, o[u].y * inv)
-                                         : pack_f16(o[u].x * inv, o[u].y * inv);
-            const uint32_t hi = FMT == 1 ? pack_bf16(o[u].z * inv, o[u].w * inv)
-                                         : pack_f16(o[u].z * inv, o[u].w * inv);
-            reinterpret_cast<uint2*>(orow)[x[u]] = make_uint2(lo, hi);
-          }
-        }
+        if (rows <= 16)
+          fwd_join<1, 8>(row, total, rows, c_first, c_last, part_row, finish);
+        else
+          fwd_join<4, 2>(row, total, rows, c_first, c_last, part_row, finish);
       }
     }
   }
@@ -881,18 +888,17 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
   static_assert(TILES * D + NB * kOpsBN <= 512, "TMEM holds 512 columns");
 
   __shared__ FwdShared sh;
-  __shared__ float2 join_ml[STREAM ? TILES * 128 : 1];
   extern __shared__ uint8_t dyn_smem[];
   const uint32_t base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
   const uint32_t q_smem = base;
   const uint32_t k_smem = q_smem + TILES * G::Q_BYTES;
-  const uint32_t v_smem = k_smem + args.stages * G::KV_BYTES;
+  const uint32_t v_smem = k_smem + args.k_stages * G::KV_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&sh.q_full), 1);
     mbar_init(smem_u32(&sh.q_empty), 1);
-    for (int s = 0; s < args.stages; ++s) {
+    for (int s = 0; s < kFwdMaxStages; ++s) {
       mbar_init(smem_u32(&sh.k_full[s]), 1);
       mbar_init(smem_u32(&sh.k_empty[s]), 1);
       mbar_init(smem_u32(&sh.v_full[s]), 1);
@@ -935,7 +941,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
       fwd_mma<FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
   } else {
     if constexpr (TILES == 2) fwd_regs_inc<kFwdHighRegs>();
-    fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, join_ml, tmem, warp, lane);
+    fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -1028,7 +1034,13 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   a.o_head = p.o_head;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.spans = fwd_spans(g);
-  a.stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
+  // Two Q tiles of D = 128 leave room for five slots.  V gets three: PV of a
+  // block frees its slot one step before the slot's next block is needed, S
+  // of a block two steps before.
+  a.v_stages = kFwdMaxStages;
+  a.k_stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
+  a.wide = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0 && p.o_batch % 16 == 0 &&
+           p.o_token % 16 == 0 && p.o_head % 16 == 0;
   a.err = c.err;
   const int64_t items = static_cast<int64_t>(a.spans) * g.batch * g.heads_kv;
   if (items > (1ll << 31) - 1024) return GPO_BAD_ARGS;
@@ -1044,7 +1056,7 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   }
   auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES>;
   const uint32_t dyn =
-      (TILES * 128u + 2u * static_cast<uint32_t>(a.stages) * kOpsBN) * D * 2u + 1024u;
+      (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN) * D * 2u + 1024u;
   gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
   kern<<<static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream>>>(mq, mk, mv, a);
