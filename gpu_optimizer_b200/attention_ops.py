@@ -164,21 +164,36 @@ def _window_args(sizes, q, k, v, out, lse, grads=4 * _NO_HEADS, workspace=(0, 0)
     return a
 
 
+def _written(name: str, t: torch.Tensor, shape, dtype, device) -> None:
+    _check(name, t, len(shape), dtype, device)
+    if t.shape != shape or not (t.is_contiguous() if dtype is torch.float32 else _in_place(t)):
+        raise KernelBuildError(f"{name} must have shape {tuple(shape)}, its rows contiguous and "
+                               f"16-byte aligned")
+
+
 def window_attention_forward(q, k, v, *, window: int | None = None, sinks: int = 0,
-                             scale: float | None = None):
+                             scale: float | None = None, out=None, lse=None):
     """(out, lse): attention of q over k, v, and each row's log-sum-exp of
-    scaled scores, fp32 (batch, q_len, heads_q)."""
+    scaled scores, fp32 (batch, q_len, heads_q).  ``out`` and ``lse`` may name
+    the tensors to write."""
     sizes = _window_sizes(q, k, v, window, sinks, scale)
     q, k, v = _readable(q), _readable(k), _readable(v)
-    out = q.new_empty(q.shape)
-    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    if out is None:
+        out = q.new_empty(q.shape)
+    else:
+        _written("out", out, q.shape, q.dtype, q.device)
+    if lse is None:
+        lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    else:
+        _written("lse", lse, q.shape[:3], torch.float32, q.device)
     _launch("gpo_window_attention", _window_args(sizes, q, k, v, out, lse), q.device)
     return out, lse
 
 
 def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = None,
-                              sinks: int = 0, scale: float | None = None):
+                              sinks: int = 0, scale: float | None = None, grads=None):
     """(dq, dk, dv) from the output's gradient and what the forward returned.
+    ``grads`` may name the three tensors to write.
 
     Sums run in a fixed order: the same inputs give the same bits.
     """
@@ -194,7 +209,12 @@ def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = N
     q, k, v, out, dout = (_readable(q), _readable(k), _readable(v), _readable(out),
                           _readable(dout))
     lse = lse.contiguous()
-    dq, dk, dv = q.new_empty(shape), q.new_empty(k.shape), q.new_empty(k.shape)
+    if grads is None:
+        dq, dk, dv = q.new_empty(shape), q.new_empty(k.shape), q.new_empty(k.shape)
+    else:
+        dq, dk, dv = grads
+        for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            _written(name, t, like.shape, q.dtype, device)
     grads = (*_heads(dout), *_heads(dq), *_heads(dk), *_heads(dv))
     size = _workspace_bytes("gpo_window_workspace", _window_args(sizes, q, k, v, out, lse))
     work = torch.empty(max(1, size), dtype=torch.uint8, device=device)
@@ -324,16 +344,80 @@ class PagedAttention:
         if out is None:
             out = q.new_empty(q.shape)
         else:
-            _check("out", out, 3, self.dtype, self.device)
-            if out.shape != q.shape or not _in_place(out):
-                raise KernelBuildError(f"out must have q's shape {tuple(q.shape)}, its rows "
-                                       "contiguous and 16-byte aligned")
+            _written("out", out, q.shape, self.dtype, self.device)
         if lse is not None:
-            _check("lse", lse, 2, torch.float32, self.device)
-            if lse.shape != q.shape[:2] or not lse.is_contiguous():
-                raise KernelBuildError(f"lse must be a contiguous {tuple(q.shape[:2])} tensor")
+            _written("lse", lse, q.shape[:2], torch.float32, self.device)
         a = self._fill(q.shape[0], k_pages, v_pages, page_table, q_start, kv_len,
                        0 if lse is None else lse.data_ptr())
         _PAGED_HEADS.pack_into(a, _lib.GpoPagedArgs.q.offset, *_heads(q), *_heads(out))
         _launch("gpo_paged_attention", a, self.device)
         return out
+
+
+# ------------------------------------------------------- runner.build_callable
+# Candidates of these operators are fixed by their problem: a config holds
+# dtype, window (0: none) and sinks, and the library picks the variant.  The
+# shapes are (batch, q_len, kv_len, heads_q, heads_kv, head_dim) and, paged,
+# (seqs, max_q, page_size, heads_q, heads_kv, head_dim).
+OPERATOR_INPUTS = {
+    "attention_window": ("q", "k", "v"),
+    "attention_window_grad": ("dout", "q", "k", "v", "out", "lse"),
+    "attention_paged": ("q", "k_pages", "v_pages", "page_table", "q_start", "kv_len"),
+    "cache_append": ("k", "v", "k_pages", "v_pages", "page_table", "q_start", "kv_len"),
+}
+_KERNELS = {"attention_window": "attn_fwd_kernel<dense>",
+            "attention_window_grad": "attn_grad_kernel",
+            "attention_paged": "attn_fwd_kernel<paged>",
+            "cache_append": "cache_append_kernel"}
+
+
+def operator_call(task: str, shape, config: dict, inputs):
+    """(fn, description, launch record) of one operator: ``fn`` launches on
+    torch's current stream and returns outputs that are allocated here."""
+    names = OPERATOR_INPUTS[task]
+    if len(inputs) != len(names):
+        raise KernelBuildError(f"{task} takes {len(names)} inputs {names}, got {len(inputs)}")
+    t = dict(zip(names, inputs))
+    want = str(config.get("dtype", "bfloat16"))
+    dtype = {"float16": torch.float16, "bfloat16": torch.bfloat16}.get(want)
+    if dtype is None:
+        raise KernelBuildError(f"{task}: dtype must be float16 or bfloat16, got {want!r}")
+    if len(shape) != 6:
+        raise KernelBuildError(f"{task}: shape needs 6 values, got {tuple(shape)}")
+    for name in names:
+        if not isinstance(t[name], torch.Tensor) or not t[name].is_cuda:
+            raise KernelBuildError("inputs must be CUDA tensors")
+    first = t[names[0]]
+    if first.dtype is not dtype:
+        raise KernelBuildError(f"input dtype {first.dtype} does not match config dtype {dtype}")
+    mask = {"window": int(config.get("window", 0)) or None, "sinks": int(config.get("sinks", 0))}
+    if task.startswith("attention_window"):
+        b, q_len, kv_len, hq, hk, dim = shape
+        for name, s in (("q", (b, q_len, hq, dim)), ("k", (b, kv_len, hk, dim))):
+            if tuple(t[name].shape) != s:
+                raise KernelBuildError(f"{name} has shape {tuple(t[name].shape)}, expected {s}")
+        if task == "attention_window":
+            out = t["q"].new_empty(t["q"].shape)
+            lse = out.new_empty(out.shape[:3], dtype=torch.float32)
+
+            def fn():
+                return window_attention_forward(*inputs, out=out, lse=lse, **mask)[0]
+        else:
+            grads = tuple(t[n].new_empty(t[n].shape) for n in ("q", "k", "v"))
+
+            def fn():
+                return window_attention_backward(*inputs, grads=grads, **mask)
+    else:
+        seqs, max_q, page_size, hq, hk, dim = shape
+        plan = PagedAttention(heads_q=hq, heads_kv=hk, head_dim=dim, page_size=page_size,
+                              max_seqs=seqs, max_q=max_q, dtype=dtype, device=first.device, **mask)
+        if task == "attention_paged":
+            out = first.new_empty(first.shape)
+
+            def fn():
+                return plan.attend(*inputs, out=out)
+        else:
+            def fn():
+                plan.append(*inputs)
+                return t["k_pages"], t["v_pages"]
+    return fn, f"b200 {_KERNELS[task]}", {"kernel": _KERNELS[task], **config}

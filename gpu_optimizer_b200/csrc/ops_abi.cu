@@ -255,7 +255,7 @@ gpo_status gpo_window_attention_grad(const gpo_window_args* a, void* stream, cha
     AttnProblem p{};
     Refusal r;
     if (!dense_problem(*a, true, p, r)) return refuse(r, log, cap);
-    if (a->batch == 0) return GPO_OK;
+    if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return GPO_OK;
     AttnGradProblem gp{};
     const int64_t b = a->batch, q = a->q_len, n = a->kv_len;
     if (q > 0) {

@@ -103,8 +103,17 @@ def _output_for(task: str, shape: Sequence[int], inputs, dtype: str) -> torch.Te
 
 def build_callable(task: str, shape: Sequence[int], config: Config,
                    inputs: tuple[torch.Tensor, ...]) -> KernelCallable:
-    """Construct the launcher for one candidate.  Raises KernelBuildError."""
+    """Construct the launcher for one candidate.  Raises KernelBuildError.
+
+    Operator names (``attention_ops.OPERATOR_INPUTS``) are built too; their
+    ``fn`` returns the operator's outputs.
+    """
     shape = tuple(int(s) for s in shape)
+    if task not in _TASK_INPUTS:
+        from . import attention_ops
+
+        if task in attention_ops.OPERATOR_INPUTS:
+            return KernelCallable(*attention_ops.operator_call(task, shape, config, inputs))
     mod = compile_module(task, shape, config)
     want = TORCH_DTYPES[str(config.get("dtype", "float32"))]
     if len(inputs) != _TASK_INPUTS[task]:
