@@ -7,6 +7,8 @@ into ``_build/`` at the repository root, the kernel sources are embedded for
 ``gpo_source`` (``_build/gpo_sources.inc``), and the objects are linked with
 the static CUDA runtime into ``gpu_optimizer_b200/libgpo.so``.  A unit is
 rebuilt only when it, or a header it includes, is newer than its object.
+The operators' Python binding (``csrc/py_ops.cpp``, host C++ on torch's
+headers) becomes ``gpu_optimizer_b200/_ops.so`` next to it.
 """
 
 from __future__ import annotations
@@ -24,6 +26,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libgpo.so"
+BINDING = PKG / "_ops.so"
 HEADERS = [CSRC / "gpo_common.cuh", CSRC / "gpo_internal.h", ROOT / "include" / "gpo.h"]
 OPS_HEADER = CSRC / "attn_ops.cuh"  # of the *_ops.cu units and ops_abi.cu
 
@@ -110,7 +113,37 @@ def build(jobs: int | None = None, verbose: bool = False, force: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}{r.stderr}")
         os.replace(tmp, LIB)
+    build_binding(verbose, force)
     return LIB
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> Path:
+    """Compile the operators' Python binding against the installed torch."""
+    src = CSRC / "py_ops.cpp"
+    if not force and not _stale(BINDING, src, [ROOT / "include" / "gpo.h"]):
+        return BINDING
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [base / "include", base / "include" / "torch" / "csrc" / "api" / "include",
+                cuda / "include", sysconfig.get_paths()["include"]]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_ops",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in includes), f"-I{ROOT / 'include'}", str(src), "-o", str(tmp),
+           f"-L{base / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           f"-L{PKG}", "-l:libgpo.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose and (r.stdout or r.stderr):
+        print(r.stdout + r.stderr, file=sys.stderr)
+    if r.returncode != 0:
+        raise RuntimeError(f"binding build failed:\n{r.stdout}{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 def main() -> None:
