@@ -26,7 +26,8 @@
 // Whole units (many of them) are dealt out in rounds, the longest rows first
 // and every other round backwards.  Few units (STREAM, paged only) are cut: all units' blocks form one
 // line, and every CTA takes an equal stretch of it, whatever the lengths of
-// the sequences, which only the device knows.  A unit that lies in one
+// the sequences, which only the device knows (or an equal number of whole
+// units, where that takes no longer).  A unit that lies in one
 // stretch is finished by its CTA; of one that is cut, every CTA writes its
 // part (O unnormalised, maximum, sum) to the workspace and the CTA that
 // arrives last joins the parts in their order.
@@ -40,6 +41,7 @@ constexpr int kFwdMaxStages = 3;       // slots of the K ring and of the V ring
 constexpr int kFwdSBufs = 3;           // S/P buffers (TILES = 1)
 constexpr float kFwdRescale = 8.0f;    // see the softmax
 constexpr int kFwdMaxCtas = 160;       // CTAs that a workspace has room for
+constexpr int kFwdCutCost = 5;         // blocks' time that writing and joining parts takes
 constexpr int kFwdStreamPairs = 1024;  // most (sequence, span) pairs of a cut launch
 // Registers of TILES = 2: 384 threads launch at 168; 128 * 88 + 256 * 208 is
 // the same total (a softmax thread holds a row of 128 scores).
@@ -58,6 +60,8 @@ struct FwdShared {
   // cut launches: where this CTA's stretch begins
   int64_t line_pos, line_end, line_len;
   int64_t warp_sum[8];
+  int warp_units[8], warp_longest[8];
+  bool line_whole;  // positions count units, not blocks
   int line_pair, line_head, line_off;
   int last[2];
   uint32_t tmem_base;
@@ -111,6 +115,7 @@ struct FwdWalk {
   int item, turn;     // whole units: first item of the CTA's turn
   int64_t pos, end;   // cut: positions in the line of blocks
   int pair, head, off, n, known;
+  bool whole;
 
   __device__ __forceinline__ FwdWalk(const FwdArgs& args, const FwdShared& sh) : a(args) {
     item = 0;
@@ -121,6 +126,7 @@ struct FwdWalk {
       pair = sh.line_pair;
       head = sh.line_head;
       off = sh.line_off;
+      whole = sh.line_whole;
       known = -1;
       n = 0;
     }
@@ -168,9 +174,9 @@ struct FwdWalk {
       s.unit = pair * g.heads_kv + head;
       s.line0 = pos - off;
       s.i0 = off;
-      s.i1 = static_cast<int>(min(static_cast<int64_t>(n), off + (end - pos)));
+      s.i1 = whole ? n : static_cast<int>(min(static_cast<int64_t>(n), off + (end - pos)));
       s.whole = s.i0 == 0 && s.i1 == n;
-      pos += s.i1 - s.i0;
+      pos += whole ? 1 : s.i1 - s.i0;
       off = s.i1;
       if (off == n) {
         off = 0;
@@ -214,7 +220,9 @@ __device__ __forceinline__ void fwd_stretch(const FwdArgs& a, FwdShared& sh) {
   const int tid = threadIdx.x, lane = tid & 31;
   FwdWalk<PAGED, false, TILES> w(a, sh);
   int cnt[kFwdStreamPairs / 256];
-  int64_t mine = 0;
+  // blocks, units (times heads) and the longest unit
+  int64_t blocks = 0;
+  int units = 0, longest = 0;
   if (tid < 256) {
 #pragma unroll
     for (int i = 0; i < kFwdStreamPairs / 256; ++i) {
@@ -223,42 +231,71 @@ __device__ __forceinline__ void fwd_stretch(const FwdArgs& a, FwdShared& sh) {
       if (i < per && r < pairs) {
         w.place(r);
         cnt[i] = w.s.t0 < w.s.t1 ? max(1, w.s.blk.n) : 0;
-        mine += cnt[i];
+        blocks += cnt[i];
+        units += cnt[i] > 0 ? 1 : 0;
+        longest = max(longest, cnt[i]);
       }
     }
   }
-  int64_t incl = mine;
+  int64_t incl = blocks;
+  int incl_u = units;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
+    const int up_u = __shfl_up_sync(0xffffffffu, incl_u, o);
+    if (lane >= o) {
+      incl += up;
+      incl_u += up_u;
+    }
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
   }
-  if (tid < 256 && lane == 31) sh.warp_sum[tid >> 5] = incl;
+  if (tid < 256 && lane == 31) {
+    sh.warp_sum[tid >> 5] = incl;
+    sh.warp_units[tid >> 5] = incl_u;
+    sh.warp_longest[tid >> 5] = longest;
+  }
   __syncthreads();
-  int64_t before = incl - mine, total = 0;
+  int64_t before = incl - blocks, total = 0;
+  int before_u = incl_u - units, total_u = 0;
+  longest = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (i < (tid >> 5)) before += sh.warp_sum[i];
+    if (i < (tid >> 5)) {
+      before += sh.warp_sum[i];
+      before_u += sh.warp_units[i];
+    }
     total += sh.warp_sum[i];
+    total_u += sh.warp_units[i];
+    longest = max(longest, sh.warp_longest[i]);
   }
   total *= g.heads_kv;
-  const int64_t len = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t all_u = static_cast<int64_t>(total_u) * g.heads_kv;
+  const int64_t ctas = gridDim.x;
+  // Whole units where that takes no longer than cut ones and their joins.
+  const bool whole = (all_u + ctas - 1) / ctas * longest <= (total + ctas - 1) / ctas + kFwdCutCost;
+  if (whole) {
+    before = before_u;
+    total = all_u;
+  }
+  const int64_t len = (total + ctas - 1) / ctas;
   const int64_t p0 = min(total, len * blockIdx.x), p1 = min(total, p0 + len);
   if (tid == 0) {
     sh.line_pos = p0;
     sh.line_end = p1;
     sh.line_len = len;
+    sh.line_whole = whole;
   }
   if (tid < 256) {
 #pragma unroll
     for (int i = 0; i < kFwdStreamPairs / 256; ++i) {
-      const int64_t b0 = before * g.heads_kv, b1 = b0 + static_cast<int64_t>(cnt[i]) * g.heads_kv;
+      const int c = whole ? (cnt[i] > 0 ? 1 : 0) : cnt[i];
+      const int64_t b0 = before * g.heads_kv, b1 = b0 + static_cast<int64_t>(c) * g.heads_kv;
       if (p0 < p1 && p0 >= b0 && p0 < b1) {
         sh.line_pair = tid * per + i;
-        sh.line_head = static_cast<int>((p0 - b0) / cnt[i]);
-        sh.line_off = static_cast<int>((p0 - b0) % cnt[i]);
+        sh.line_head = static_cast<int>((p0 - b0) / c);
+        sh.line_off = static_cast<int>((p0 - b0) % c);
       }
-      before += cnt[i];
+      before += c;
     }
   }
 }
@@ -926,11 +963,16 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
     tmem_alloc(smem_u32(&sh.tmem_base), 512);
     tmem_relinquish();
   }
-  if constexpr (STREAM) fwd_stretch<PAGED, TILES>(args, sh);
+  let_next_start();
+  if constexpr (STREAM) {
+    wait_for_previous();
+    fwd_stretch<PAGED, TILES>(args, sh);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
+  if constexpr (!STREAM) wait_for_previous();
 
   if (warp < 4) {
     if constexpr (TILES == 2) fwd_regs_dec<kFwdLowRegs>();
@@ -1059,8 +1101,8 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
       (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN) * D * 2u + 1024u;
   gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
-  kern<<<static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream>>>(mq, mk, mv, a);
-  return launch_status();
+  return launch_in_order(kern, static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream, mq,
+                         mk, mv, a);
 }
 
 template <typename T, int FMT, int D>

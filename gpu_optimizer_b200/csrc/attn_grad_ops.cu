@@ -72,6 +72,8 @@ __device__ __forceinline__ float* grad_stats(const GradArgs& a, int b, int h, in
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) {
   const AttnGeom& g = a.geom;
+  let_next_start();
+  wait_for_previous();
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.next = 0u;
   if (g.tiles == 0) return;
   constexpr int LPR = D / 8, RPW = 32 / LPR;  // lanes per row, rows per warp
@@ -876,6 +878,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
+  let_next_start();
+  wait_for_previous();
   if (warp == 0) {
     if (elect_one()) grad_producer<D, 0>(args, sh, maps, base);
   } else if (warp == 3) {
@@ -906,6 +910,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 template <typename T, int D>
 __global__ void __launch_bounds__(2 * D) attn_grad_join_kernel(const GradArgs a) {
   const AttnGeom& g = a.geom;
+  let_next_start();
+  wait_for_previous();
   const int key = blockIdx.x % g.sinks, bh = blockIdx.x / g.sinks;
   const int h = bh % g.heads_kv, b = bh / g.heads_kv;
   const int x = threadIdx.x;
@@ -995,20 +1001,19 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   a.items = static_cast<int>(q_items + kv_items);
   if (a.items == 0) return GPO_OK;
   const int sms = c.sm_count > 0 ? c.sm_count : 148;
-  attn_grad_stats_kernel<T, D>
-      <<<static_cast<unsigned>(std::max<int64_t>(1, q_items)), 256, 0, c.stream>>>(a);
-  if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
+  gpo_status s = launch_in_order(attn_grad_stats_kernel<T, D>,
+                                 static_cast<unsigned>(std::max<int64_t>(1, q_items)), 256, 0,
+                                 c.stream, a);
+  if (s != GPO_OK) return s;
   auto kern = attn_grad_kernel<T, FMT, D>;
   constexpr uint32_t dyn = GradGeom<D>::BYTES;
-  const gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
+  s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
-  kern<<<static_cast<unsigned>(std::min(a.items, sms)), kGradThreads, dyn, c.stream>>>(mq, mdo, mk,
-                                                                                      mv, a);
-  if (launch_status() != GPO_OK) return GPO_LAUNCH_ERROR;
-  if (pl.sink_tiles > 0)
-    attn_grad_join_kernel<T, D>
-        <<<static_cast<unsigned>(heads * g.sinks), 2 * D, 0, c.stream>>>(a);
-  return launch_status();
+  s = launch_in_order(kern, static_cast<unsigned>(std::min(a.items, sms)), kGradThreads, dyn,
+                      c.stream, mq, mdo, mk, mv, a);
+  if (s != GPO_OK || pl.sink_tiles == 0) return s;
+  return launch_in_order(attn_grad_join_kernel<T, D>, static_cast<unsigned>(heads * g.sinks), 2 * D,
+                         0, c.stream, a);
 }
 
 }  // namespace

@@ -19,6 +19,8 @@ struct AppendArgs {
 
 __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const AttnGeom& g = a.geom;
+  let_next_start();
+  wait_for_previous();
   const int per_token = g.heads_kv * a.vecs;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t t64 = i / per_token;
@@ -70,8 +72,7 @@ gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c) {
   const uint64_t n = static_cast<uint64_t>(p.geom.tokens) * p.geom.heads_kv * a.vecs;
   const uint64_t blocks = cdiv(n, 256);
   if (blocks > 0x7fffffffull) return GPO_BAD_ARGS;
-  cache_append_kernel<<<static_cast<unsigned>(blocks), 256, 0, c.stream>>>(a);
-  return launch_status();
+  return launch_in_order(cache_append_kernel, static_cast<unsigned>(blocks), 256, 0, c.stream, a);
 }
 
 }  // namespace gpo
