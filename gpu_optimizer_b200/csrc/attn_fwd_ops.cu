@@ -11,7 +11,7 @@
 //   warp 0     TMA of Q and of the K ring
 //   warp 3     TMA of the V ring; clears V rows behind a sequence's last key
 //   warp 1     MMA issuer; P overlays S in TMEM as 16-bit pairs
-//   warp 2     TMEM owner
+//   warp 2     TMEM owner; walks the CTA's stretches and hands them out
 //   warps 4-7  softmax and epilogue of tile 0, thread = query row = TMEM
 //   warps 8-11 lane; of tile 1
 // TILES = 2 (more than 128 rows per sequence and kv head): both tiles share
@@ -49,7 +49,37 @@ constexpr int kFwdLowRegs = 88, kFwdHighRegs = 208;
 static_assert(128 * kFwdLowRegs + 256 * kFwdHighRegs <= 168 * 384,
               "register split exceeds the launch's registers");
 
+// A stretch of a unit: blocks [i0, i1) of the n that its span sees.
+struct FwdSeg {
+  int b, h, t0, t1;  // tokens [t0, t1) of the span
+  AttnSeq seq;
+  AttnBlocks blk;
+  int i0, i1;
+  int64_t line0;  // cut launches: position of the unit's first block
+  int unit;
+  bool whole;
+};
+
+// Tile t of a stretch: its tokens and which of the span's blocks it sees.
+struct FwdTile {
+  int t0, t1, first, last, sinks;
+  __device__ __forceinline__ bool sees(int block) const {
+    return block <= last && (block >= first || block < sinks);
+  }
+};
+
+// What warp 2 hands to the other roles (a single thread takes 3500 cycles to
+// work a stretch out, which every role had to wait for when each did it).
+struct FwdWork {
+  FwdSeg seg;
+  FwdTile tile[2];
+  int more;  // 0: no stretch, the CTA is done
+};
+
 struct FwdShared {
+  FwdWork work[2];
+  uint64_t work_full[2], work_empty[2];
+
   uint64_t q_full, q_empty;
   uint64_t k_full[kFwdMaxStages], k_empty[kFwdMaxStages];
   uint64_t v_full[kFwdMaxStages], v_empty[kFwdMaxStages];
@@ -96,18 +126,7 @@ struct RingPos2 {
   }
 };
 
-// A stretch of a unit: blocks [i0, i1) of the n that its span sees.
-struct FwdSeg {
-  int b, h, t0, t1;  // tokens [t0, t1) of the span
-  AttnSeq seq;
-  AttnBlocks blk;
-  int i0, i1;
-  int64_t line0;  // cut launches: position of the unit's first block
-  int unit;
-  bool whole;
-};
-
-// The CTA's stretches in order; every role walks them by itself.
+// The CTA's stretches in order.
 template <bool PAGED, bool STREAM, int TILES>
 struct FwdWalk {
   const FwdArgs& a;
@@ -191,14 +210,6 @@ struct FwdWalk {
   }
 };
 
-// Tile t of a stretch: its tokens and which of the span's blocks it sees.
-struct FwdTile {
-  int t0, t1, first, last, sinks;
-  __device__ __forceinline__ bool sees(int block) const {
-    return block <= last && (block >= first || block < sinks);
-  }
-};
-
 __device__ __forceinline__ FwdTile fwd_tile(const AttnGeom& g, const FwdSeg& s, int t) {
   FwdTile f;
   f.t0 = s.t0 + t * g.tpt;
@@ -208,6 +219,46 @@ __device__ __forceinline__ FwdTile fwd_tile(const AttnGeom& g, const FwdSeg& s, 
   f.sinks = b.sink_blocks;
   f.last = b.n > 0 ? b.first + b.n - b.sink_blocks - 1 : -1;
   return f;
+}
+
+// Warp 2: works out the CTA's stretches, up to two ahead of their readers.
+template <bool PAGED, bool STREAM, int TILES>
+__device__ __forceinline__ void fwd_schedule(const FwdArgs& args, FwdShared& sh) {
+  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
+  for (int n = 0;; ++n) {
+    if (n >= 2 && !mbar_wait(smem_u32(&sh.work_empty[n & 1]), ((n >> 1) - 1) & 1u, &sh.abort,
+                             args.err, kErrWaitProducer))
+      return;
+    FwdWork& to = sh.work[n & 1];
+    const bool more = w.next();
+    to.more = more ? 1 : 0;
+    if (more) {
+      to.seg = w.s;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) to.tile[t] = fwd_tile(args.geom, w.s, t);
+    }
+    mbar_arrive(smem_u32(&sh.work_full[n & 1]));
+    if (!more) return;
+  }
+}
+
+// The n-th stretch for one role: false when there is none (or a wait failed).
+template <bool WARP>
+__device__ __forceinline__ bool fwd_take(FwdShared& sh, uint32_t& n, FwdSeg& s, unsigned int* err,
+                                         uint32_t site, bool& ok) {
+  const int i = n & 1u;
+  ok = mbar_wait(smem_u32(&sh.work_full[i]), (n >> 1) & 1u, &sh.abort, err, site);
+  if (WARP) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  const bool more = *reinterpret_cast<volatile int*>(&sh.work[i].more) != 0;
+  if (more) s = sh.work[i].seg;
+  return more;
+}
+template <bool WARP>
+__device__ __forceinline__ void fwd_taken(FwdShared& sh, uint32_t& n) {
+  if (WARP) __syncwarp();
+  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sh.work_empty[n & 1u]));
+  ++n;
 }
 
 // Cut launches: the blocks of every (sequence, span) pair are counted, and
@@ -376,7 +427,7 @@ struct FwdGeom {
 // ---------------------------------------------------------------- producer
 // K ring and Q (is_k), or V ring.  The whole warp runs the loop: each lane
 // loads one box of a block.
-template <int D, bool PAGED, bool STREAM, int TILES>
+template <int D, bool PAGED, int TILES>
 __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
                                              const CUtensorMap* tma_q, const CUtensorMap* map,
                                              uint32_t q_smem, uint32_t ring, bool is_k, int lane) {
@@ -390,9 +441,10 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
   bool ok = true;
   int issued = 0, q_loads = 0;
   RingPos2 pos;
-  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
-  while (ok && w.next()) {
-    const FwdSeg& s = w.s;
+  uint32_t taken = 0;
+  FwdSeg s;
+  while (fwd_take<true>(sh, taken, s, args.err, kErrWaitProducer, ok)) {
+    fwd_taken<true>(sh, taken);
     if (s.i0 == s.i1) continue;
     if (is_k) {
       // Q of the previous stretch is free once its last S MMA is done
@@ -455,6 +507,7 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
       }
       pos.step(stages);
     }
+    if (!ok) break;
   }
   if (!ok && lane == 0) {
     // let the copies in flight land before the CTA can exit
@@ -465,7 +518,7 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
 }
 
 // -------------------------------------------------------------- MMA issuer
-template <int FMT, int D, bool PAGED, bool STREAM, int TILES>
+template <int FMT, int D, bool PAGED, int TILES>
 __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint32_t tmem,
                                         uint32_t q_smem, uint32_t k_smem, uint32_t v_smem) {
   using G = FwdGeom<D>;
@@ -513,13 +566,13 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
     }
     return true;
   };
-  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
-  uint32_t segs = 0;
+  uint32_t segs = 0, taken = 0;
+  FwdSeg s;
   if constexpr (TILES == 1) {
     constexpr int NB = kFwdSBufs, LAG = NB - 1;
     RingPos2 spos, ppos;
-    while (ok && w.next()) {
-      const FwdSeg& s = w.s;
+    while (fwd_take<false>(sh, taken, s, err, kErrWaitMma, ok)) {
+      fwd_taken<false>(sh, taken);
       const int n = s.i1 - s.i0;
       if (n == 0) continue;
       ok = wait(&sh.q_full, segs & 1u);
@@ -552,15 +605,16 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
           ppos.step(NB);
         }
       }
+      if (!ok) break;
       ++segs;
     }
   } else {
     uint32_t blocks[2] = {0u, 0u};  // blocks of each tile so far: phases of its P
     uint32_t outs[2] = {0u, 0u};    // stretches in which the tile had a block
-    while (ok && w.next()) {
-      const FwdSeg& s = w.s;
+    while (fwd_take<false>(sh, taken, s, err, kErrWaitMma, ok)) {
+      const FwdTile tile[2] = {sh.work[taken & 1u].tile[0], sh.work[taken & 1u].tile[1]};
+      fwd_taken<false>(sh, taken);
       if (s.i0 == s.i1) continue;
-      const FwdTile tile[2] = {fwd_tile(g, s, 0), fwd_tile(g, s, 1)};
       auto sees = [&](int t, int i) { return tile[t].sees(s.blk.at(i)); };
       bool begun[2] = {false, false};
       ok = wait(&sh.q_full, segs & 1u) && wait(&sh.k_full[kpos.slot], kpos.parity);
@@ -642,6 +696,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
 #pragma unroll
         for (int t = 0; t < 2; ++t) now[t] = then[t];
       }
+      if (!ok) break;
       ++segs;
     }
   }
@@ -675,10 +730,11 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
   RingPos2 spos, last_pv;     // TILES = 1: S buffers
   uint32_t blocks = 0, outs = 0;
   if (TILES == 2) spos.slot = t;
-  FwdWalk<PAGED, STREAM, TILES> w(args, sh);
-  while (ok && w.next()) {
-    const FwdSeg& s = w.s;
-    const FwdTile tile = fwd_tile(g, s, t);
+  uint32_t taken = 0;
+  FwdSeg s;
+  while (fwd_take<true>(sh, taken, s, err, kErrWaitSoftmax, ok)) {
+    const FwdTile tile = sh.work[taken & 1u].tile[t];
+    fwd_taken<true>(sh, taken);
     if (tile.t0 >= tile.t1) continue;
     const int token = tile.t0 + row_token;
     const bool live = row_token < g.tpt && token < tile.t1;
@@ -952,6 +1008,10 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
       mbar_init(smem_u32(&sh.o_full[t]), 1);
       mbar_init(smem_u32(&sh.o_free[t]), 4);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.work_full[i]), 1);
+      mbar_init(smem_u32(&sh.work_empty[i]), 3 + 4 * TILES);  // two producers, MMA, softmax warps
+    }
     mbar_init(smem_u32(&sh.drain), 1);
     sh.abort = 0;
     fence_barrier_init();
@@ -977,10 +1037,12 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
   if (warp < 4) {
     if constexpr (TILES == 2) fwd_regs_dec<kFwdLowRegs>();
     if (warp == 0 || warp == 3)
-      fwd_producer<D, PAGED, STREAM, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
-                                            warp == 0 ? k_smem : v_smem, warp == 0, lane);
+      fwd_producer<D, PAGED, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
+                                    warp == 0 ? k_smem : v_smem, warp == 0, lane);
     else if (warp == 1 && elect_one())
-      fwd_mma<FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
+      fwd_mma<FMT, D, PAGED, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
+    else if (warp == 2 && elect_one())
+      fwd_schedule<PAGED, STREAM, TILES>(args, sh);
   } else {
     if constexpr (TILES == 2) fwd_regs_inc<kFwdHighRegs>();
     fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, warp, lane);

@@ -17,11 +17,11 @@
 // sink keys' partial sums, see kv_piece.)
 //
 // Roles of the persistent kernel, one CTA per SM:
-//   warp 0     takes work items from a counter; TMA of the item's first own
-//              tile (K or Q), of ring A (Q or K) and of the row statistics
+//   warp 0     TMA of the item's first own tile (K or Q), of ring A (Q or K)
+//              and of the row statistics
 //   warp 3     TMA of the second own tile (V or dO) and of ring B (dO or V)
 //   warp 1     MMA issuer
-//   warp 2     TMEM owner
+//   warp 2     TMEM owner; takes work items from a counter and works them out
 //   warps 4-11 elementwise: thread = TMEM lane, 64 of a tile's 128 columns
 // Ring A is three tiles deep and ring B two (with D = 128 that fills shared
 // memory): a tile of A is needed by the last product of a step and again
@@ -36,8 +36,7 @@ namespace gpo {
 constexpr int kGradA = 3, kGradB = 2;  // ring depths
 constexpr int kGradThreads = 384;      // 4 service warps, 2 x 4 elementwise warps
 constexpr int kGradEwWarps = 8;
-constexpr int kGradFma = 2;             // of 4 pairs of exponentials (see exp2_to)
-constexpr int kGradReaders = 2 + kGradEwWarps;  // of an item: warp 3, warp 1, elementwise
+constexpr int kGradReaders = 3 + kGradEwWarps;  // of an item: producers, MMA, elementwise
 
 struct GradArgs {
   AttnGeom geom;
@@ -116,6 +115,25 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
 }
 
 // ------------------------------------------------------------- shared parts
+struct KvPiece {
+  int b, h, kt, piece;  // piece 0: main
+  int first, n;         // query tiles
+};
+
+struct QItem {
+  int b, h, t0, t1, tile;
+  AttnSeq seq;
+  AttnBlocks blk;
+};
+
+// A work item as warp 2 hands it to the other roles.
+struct GradWork {
+  int kind;  // 0: none left, 1: key tile, 2: query tile
+  int n;     // steps
+  KvPiece p;
+  QItem q;
+};
+
 struct GradShared {
   uint64_t own_full[2], own_empty[2];
   uint64_t a_full[kGradA], a_empty[kGradA];
@@ -127,7 +145,7 @@ struct GradShared {
   uint64_t dv_full, acc_full, acc_free;
   uint64_t item_full[2], item_empty[2];
   uint64_t drain;
-  int item[2];
+  GradWork work[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -183,17 +201,20 @@ struct GradRing {
   }
 };
 
-// The item of the CTA's it-th turn, published by warp 0 (-1: no more).
+// The CTA's it-th item for one role; false when there is none (or the wait
+// failed).
 template <bool WARP>
-__device__ __forceinline__ bool grad_next_item(GradShared& sh, int it, volatile int* abort_flag,
-                                               unsigned int* err, uint32_t site, int& item) {
-  bool ok = mbar_wait(smem_u32(&sh.item_full[it & 1]), (it >> 1) & 1u, abort_flag, err, site);
+__device__ __forceinline__ bool grad_take(GradShared& sh, uint32_t& it, GradWork& w,
+                                          unsigned int* err, uint32_t site, bool& ok) {
+  const int i = it & 1u;
+  ok = mbar_wait(smem_u32(&sh.item_full[i]), (it >> 1) & 1u, &sh.abort, err, site);
   if (WARP) ok = __all_sync(0xffffffffu, ok);
   if (!ok) return false;
-  item = *reinterpret_cast<volatile int*>(&sh.item[it & 1]);
+  w = sh.work[i];
   if (WARP) __syncwarp();
-  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sh.item_empty[it & 1]));
-  return true;
+  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&sh.item_empty[i]));
+  ++it;
+  return w.kind != 0;
 }
 
 // D[tmem, 128 x N] (+)= A B^T over 128-byte-swizzled K-major tiles of 128
@@ -250,11 +271,6 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* dst, float f, bool 
 // later ones, which see the sink keys alone; those are cut into far pieces
 // of far_tiles query tiles, so that no CTA has a longer way than the others.
 // The pieces' sums of the sink rows are joined by attn_grad_join_kernel.
-struct KvPiece {
-  int b, h, kt, piece;  // piece 0: main
-  int first, n;         // query tiles
-};
-
 __device__ __forceinline__ void kv_tile_range(const GradArgs& a, int kt, int& first, int& last) {
   const AttnGeom& g = a.geom;
   const int off = g.kv_len - g.q_len;
@@ -297,12 +313,6 @@ __device__ __forceinline__ float* kv_partial(const GradArgs& a, int b, int h, in
 }
 
 // ------------------------------------------------------------ query tiles
-struct QItem {
-  int b, h, t0, t1, tile;
-  AttnSeq seq;
-  AttnBlocks blk;
-};
-
 __device__ __forceinline__ QItem q_item(const GradArgs& a, int item) {
   const AttnGeom& g = a.geom;
   QItem it;
@@ -315,6 +325,32 @@ __device__ __forceinline__ QItem q_item(const GradArgs& a, int item) {
   it.t1 = min(it.t0 + g.tpt, g.q_len);
   it.blk = attn_blocks(g, it.seq, it.t0, it.t1);
   return it;
+}
+
+// Warp 2: takes an item once every role has begun the one before, and not
+// earlier: an item that waits in a busy CTA is one that an idle CTA lacks.
+__device__ __forceinline__ void grad_schedule(const GradArgs& args, GradShared& sh) {
+  for (int it = 0;; ++it) {
+    if (it >= 1 && !mbar_wait(smem_u32(&sh.item_empty[(it - 1) & 1]), ((it - 1) >> 1) & 1u,
+                              &sh.abort, args.err, kErrWaitProducer))
+      return;
+    const unsigned int item = atomicAdd(args.next, 1u);
+    GradWork w{};
+    if (item < static_cast<unsigned int>(args.items)) {
+      if (item < static_cast<unsigned int>(args.kv_items)) {
+        w.kind = 1;
+        w.p = kv_piece(args, static_cast<int>(item));
+        w.n = w.p.n;
+      } else {
+        w.kind = 2;
+        w.q = q_item(args, static_cast<int>(item));
+        w.n = w.q.blk.n;
+      }
+    }
+    sh.work[it & 1] = w;
+    mbar_arrive(smem_u32(&sh.item_full[it & 1]));
+    if (w.kind == 0) return;
+  }
 }
 
 struct GradMaps {
@@ -358,30 +394,13 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
   int own = 0, issued = 0, stats = 0;
   GradRing<N> pos;
   GradRing<2> st;
-  for (int it = 0; ok; ++it) {
-    int item;
-    if constexpr (SIDE == 0) {
-      // the slot's last item has been read by every other role
-      if (it >= 2 && !wait(&sh.item_empty[it & 1], ((it >> 1) - 1) & 1u)) {
-        ok = false;
-        break;
-      }
-      const int next = static_cast<int>(atomicAdd(args.next, 1u));
-      item = next < args.items ? next : -1;
-      sh.item[it & 1] = item;
-      mbar_arrive(smem_u32(&sh.item_full[it & 1]));
-    } else {
-      ok = grad_next_item<false>(sh, it, abort_flag, err, kErrWaitProducer, item);
-    }
-    if (!ok || item < 0) break;
-    const bool keys = item < args.kv_items;
-    KvPiece p{};
-    QItem qi{};
-    if (keys)
-      p = kv_piece(args, item);
-    else
-      qi = q_item(args, item);
-    const int n = keys ? p.n : qi.blk.n;
+  uint32_t taken = 0;
+  GradWork w;
+  while (grad_take<false>(sh, taken, w, err, kErrWaitProducer, ok)) {
+    const bool keys = w.kind == 1;
+    const KvPiece& p = w.p;
+    const QItem& qi = w.q;
+    const int n = w.n;
     if (n == 0) continue;
     if (own > 0 && !wait(&sh.own_empty[SIDE], (own - 1) & 1u)) {
       ok = false;
@@ -419,6 +438,7 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
         st.step();
       }
     }
+    if (!ok) break;
   }
   if (!ok) {
     // let the copies in flight land before the CTA can exit
@@ -471,12 +491,11 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
   GradRing<kGradA> a;  // next tile of ring A that has not been waited for
   GradRing<kGradB> b;
   uint32_t own = 0, cnt = 0, qcnt = 0;
-  for (int it = 0; ok; ++it) {
-    int item;
-    ok = grad_next_item<false>(sh, it, abort_flag, err, kErrWaitMma, item);
-    if (!ok || item < 0) break;
-    const bool keys = item < args.kv_items;
-    const int n = keys ? kv_piece(args, item).n : q_item(args, item).blk.n;
+  uint32_t taken = 0;
+  GradWork w;
+  while (grad_take<false>(sh, taken, w, err, kErrWaitMma, ok)) {
+    const bool keys = w.kind == 1;
+    const int n = w.n;
     if (n == 0) continue;
     const uint32_t op = own & 1u;
     if (keys) {
@@ -573,6 +592,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
         if (!more) commit(&sh.acc_full);
       }
     }
+    if (!ok) break;
     ++own;
   }
   if (!ok) {
@@ -611,12 +631,15 @@ struct GradEw {
                                     reinterpret_cast<uint32_t*>(x) + c * 32));
     tmem_wait_ld();
   }
-  // P of a pair.  The exponentials take the special function unit 1024
-  // cycles per step (16 a cycle), longer than anything else the elementwise
-  // warps do, so kGradFma of every 4 pairs run on the FMA pipe.
+  // P of a pair.  The exponentials keep the special function unit busy for
+  // 1024 cycles per step (16 a cycle).  With D = 64 that is what a step waits
+  // for, and every other pair of two runs on the FMA pipe (backward of 8192
+  // tokens, W 1024: 454 -> 402 us); with D = 128 a step waits for its MMAs,
+  // and the same exchange gained nothing (476 -> 473 us).
+  static constexpr int kFma = D == 64 ? 2 : 0;  // of 4 pairs
   static __device__ __forceinline__ void exp2_to(float (&pr)[64], int i, float2 x) {
     float2 y;
-    if ((i / 2) % 4 < kGradFma)
+    if ((i / 2) % 4 < kFma)
       y = exp2_fma<FMT == 1 ? 3 : 4>(x);
     else
       y = make_float2(ex2_approx(x.x), ex2_approx(x.y));
@@ -638,7 +661,7 @@ struct GradEw {
   }
 
   // thread = key; 64 packed query rows of the tile
-  __device__ __forceinline__ void keys(int item) {
+  __device__ __forceinline__ void keys(const KvPiece& p) {
     using G = GradGeom<D>;
     using C = GradTmem<D>;
     const AttnGeom& g = args.geom;
@@ -646,7 +669,6 @@ struct GradEw {
     const uint32_t dp_t = tmem + lane_addr + C::DP + wg * 64;
     const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
     const int off = g.kv_len - g.q_len;
-    const KvPiece p = kv_piece(args, item);
     const int k0 = p.kt * 128, key = k0 + row;
     // tokens that see this key: [key - off, key - off + window), or all
     // later ones for a sink key
@@ -768,12 +790,11 @@ struct GradEw {
   }
 
   // thread = packed query row; 64 keys of the block
-  __device__ __forceinline__ void rows(int item) {
+  __device__ __forceinline__ void rows(const QItem& it) {
     using C = GradTmem<D>;
     const AttnGeom& g = args.geom;
     const uint32_t dp_t = tmem + lane_addr + C::QDP + wg * 64;
     const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
-    const QItem it = q_item(args, item);
     const int row_token = row / g.g, row_head = row % g.g;
     const int token = it.t0 + row_token;
     const bool live = row_token < g.tpt && token < it.t1;
@@ -886,18 +907,20 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     if (elect_one()) grad_producer<D, 1>(args, sh, maps, base);
   } else if (warp == 1) {
     if (elect_one()) grad_mma<FMT, D>(args, sh, base, tmem);
+  } else if (warp == 2) {
+    if (elect_one()) grad_schedule(args, sh);
   } else if (warp >= 4) {
     const int q = warp & 3;
     GradEw<T, FMT, D> ew{args, sh, base, tmem, (warp - 4) >> 2, q * 32 + lane, lane,
                          static_cast<uint32_t>(q * 32) << 16};
-    for (int it = 0; ew.ok; ++it) {
-      int item;
-      if (!grad_next_item<true>(sh, it, &sh.abort, args.err, kErrWaitSoftmax, item) || item < 0)
-        break;
-      if (item < args.kv_items)
-        ew.keys(item);
+    uint32_t taken = 0;
+    GradWork w;
+    while (grad_take<true>(sh, taken, w, args.err, kErrWaitSoftmax, ew.ok)) {
+      if (w.kind == 1)
+        ew.keys(w.p);
       else
-        ew.rows(item);
+        ew.rows(w.q);
+      if (!ew.ok) break;
     }
   }
   tc_fence_before();

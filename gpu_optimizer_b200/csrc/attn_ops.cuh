@@ -58,7 +58,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnGeom& g, int b, unsigned i
       s.row0 = 0;
       s.q_len = 0;
       s.kv_len = 0;
-      if (threadIdx.x == 0) atomicOr(err, kErrBadLaunch);
+      atomicOr(err, kErrBadLaunch);
     }
   } else {
     s.row0 = 0;
@@ -119,15 +119,15 @@ __device__ __forceinline__ bool block_is_masked(const AttnGeom& g, const AttnSeq
 
 // 2^x of two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by
 // a polynomial of least relative error on that interval (7.5e-5 of degree 3,
-// 2.6e-6 of degree 4; fitted by iteratively reweighted least squares), n added
-// to the exponent.  For values that are rounded to 16 bits next (degree 3:
-// bfloat16, 4: float16).  x below -126 gives at most 2^-126.
+// 2.6e-6 of degree 4; fitted by iteratively reweighted least squares), 2^n
+// multiplied in.  For values that are rounded to 16 bits next (degree 3:
+// bfloat16, 4: float16).  x below -126 gives 2^-126, NaN stays NaN.
 template <int DEGREE>
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to integer
   auto both = [](float v) { return make_float2(v, v); };
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
   const float2 n = __fadd2_rn(x, both(kRound));
   const float2 f = __fadd2_rn(x, __ffma2_rn(n, both(-1.f), both(kRound)));
   float2 p;
@@ -142,8 +142,8 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
     p = __ffma2_rn(f, p, both(0.9999993f));
   }
   // the integer n sits in the low bits of n + kRound
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+  return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3F800000u),
+                                   __uint_as_float((__float_as_uint(n.y) << 23) + 0x3F800000u)));
 }
 
 // Eight 16-bit pairs to global memory: one 32-byte store where the address
