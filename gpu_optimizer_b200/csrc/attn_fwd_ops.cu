@@ -11,13 +11,19 @@
 //   warp 0     TMA of Q and of the K ring
 //   warp 3     TMA of the V ring; clears V rows behind a sequence's last key
 //   warp 1     MMA issuer; P overlays S in TMEM as 16-bit pairs
-//   warp 2     TMEM owner; walks the CTA's stretches and hands them out
+//   warp 2     TMEM owner; walks the CTA's stretches and hands them out; sends
+//              staged tiles of O to memory
 //   warps 4-7  softmax and epilogue of tile 0, thread = query row = TMEM
 //   warps 8-11 lane; of tile 1
 // TILES = 2 (more than 128 rows per sequence and kv head): both tiles share
 // every K/V block; the issuer alternates them, so that one tile's softmax
 // hides behind the other's MMAs.  TILES = 1 (single tokens, short chunks):
 // bound by the K/V bytes; three S buffers let S run two blocks ahead of PV.
+//
+// With TILES = 2 a whole tile of O leaves through a staging tile in shared
+// memory and TMA.  (Stores straight from the rows' threads touch 32 lines
+// each; while they drain, some 2500 cycles per tile, no barrier of the SM
+// advances.)
 //
 // Only blocks with a visible key are loaded.  A page that ends inside a
 // block is loaded as boxes of its own rows; boxes without a key are asked
@@ -86,6 +92,8 @@ struct FwdShared {
   uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared behind the last key
   uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], p_half[2], pv_done[kFwdSBufs];
   uint64_t o_full[2], o_free[2];
+  uint64_t stage_full, stage_empty;  // one staging tile for both tiles of O
+  int stage_at[8][3];                // batch, head, first row of the coming uses
   uint64_t drain;
   // cut launches: where this CTA's stretch begins
   int64_t line_pos, line_end, line_len;
@@ -221,25 +229,74 @@ __device__ __forceinline__ FwdTile fwd_tile(const AttnGeom& g, const FwdSeg& s, 
   return f;
 }
 
-// Warp 2: works out the CTA's stretches, up to two ahead of their readers.
-template <bool PAGED, bool STREAM, int TILES>
-__device__ __forceinline__ void fwd_schedule(const FwdArgs& args, FwdShared& sh) {
+// Whether tile f of a stretch leaves through the staging tile: a whole
+// unit's, of full height where the tensor would go on behind it.
+template <bool PAGED, bool STREAM>
+__device__ __forceinline__ bool fwd_staged(const AttnGeom& g, const FwdSeg& s, const FwdTile& f) {
+  return f.t0 < f.t1 && (!STREAM || s.whole) && (!PAGED || f.t1 - f.t0 == g.tpt);
+}
+
+// Warp 2: works out the CTA's stretches, up to two ahead of their readers,
+// and stores the staging tile whenever a warpgroup has filled it.
+template <int D, bool PAGED, bool STREAM, int TILES>
+__device__ __forceinline__ void fwd_schedule(const FwdArgs& args, FwdShared& sh,
+                                             const CUtensorMap* tma_o, uint32_t stage) {
   FwdWalk<PAGED, STREAM, TILES> w(args, sh);
-  for (int n = 0;; ++n) {
-    if (n >= 2 && !mbar_wait(smem_u32(&sh.work_empty[n & 1]), ((n >> 1) - 1) & 1u, &sh.abort,
-                             args.err, kErrWaitProducer))
-      return;
-    FwdWork& to = sh.work[n & 1];
-    const bool more = w.next();
-    to.more = more ? 1 : 0;
-    if (more) {
-      to.seg = w.s;
+  bool more = true;
+  uint32_t uses = 0, stored = 0;  // of the staging tile: planned, done
+  unsigned long long idle_since = globaltimer_ns();
+  for (uint32_t n = 0, poll = 1; more || stored < uses; ++poll) {
+    bool moved = false;
+    if (more && (n < 2 || mbar_test_wait(smem_u32(&sh.work_empty[n & 1]), ((n >> 1) - 1) & 1u))) {
+      FwdWork& to = sh.work[n & 1];
+      more = w.next();
+      to.more = more ? 1 : 0;
+      if (more) {
+        to.seg = w.s;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) to.tile[t] = fwd_tile(args.geom, w.s, t);
+        for (int t = 0; t < TILES; ++t) {
+          const FwdTile f = fwd_tile(args.geom, w.s, t);
+          to.tile[t] = f;
+          if (TILES == 2 && fwd_staged<PAGED, STREAM>(args.geom, w.s, f)) {
+            int* at = sh.stage_at[uses & 7];
+            at[0] = PAGED ? 0 : w.s.b;
+            at[1] = w.s.h;
+            at[2] = w.s.seq.row0 + f.t0;
+            ++uses;
+          }
+        }
+      }
+      mbar_arrive(smem_u32(&sh.work_full[n & 1]));
+      ++n;
+      moved = true;
     }
-    mbar_arrive(smem_u32(&sh.work_full[n & 1]));
-    if (!more) return;
+    if (TILES == 2 && stored < uses && mbar_test_wait(smem_u32(&sh.stage_full), stored & 1u)) {
+      const int* at = sh.stage_at[stored & 7];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        tma_store_5d(tma_o, stage + c * 128 * 128, c * 64, 0, at[1], at[2], at[0]);
+      bulk_commit();
+      bulk_wait_read();
+      mbar_arrive(smem_u32(&sh.stage_empty));
+      ++stored;
+      moved = true;
+    }
+    if (moved) {
+      idle_since = globaltimer_ns();
+    } else {
+      __nanosleep(64);
+      // The longest pause between two stretches is the work on one of them;
+      // the roles at it have their own limit per wait and raise the flag.
+      if ((poll & 255u) == 0 &&
+          (*reinterpret_cast<volatile int*>(&sh.abort) ||
+           globaltimer_ns() - idle_since > 16 * kWaitLimitNs)) {
+        atomicOr(args.err, kErrWaitProducer);
+        sh.abort = 1;
+        break;
+      }
+    }
   }
+  if (TILES == 2) bulk_wait();  // the last stores are out
 }
 
 // The n-th stretch for one role: false when there is none (or a wait failed).
@@ -527,7 +584,6 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
   constexpr uint32_t IDESC_O = make_idesc(FMT, 128, D, false, true);
   constexpr uint32_t S_COL = TILES * D;  // S/P buffers behind the O tiles
   constexpr uint64_t HI = smem_desc_hi(8 * SW, SW);
-  const AttnGeom& g = args.geom;
   unsigned int* err = args.err;
   volatile int* abort_flag = &sh.abort;
   // Between two MMA groups this thread does as little as it can: descriptor
@@ -708,8 +764,8 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
 
 // ---------------------------------------------------- softmax and epilogue
 template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
-__device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, uint32_t tmem,
-                                            int warp, int lane) {
+__device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, uint32_t stage,
+                                            uint32_t tmem, int warp, int lane) {
   constexpr int BN = kOpsBN;
   constexpr uint32_t S_COL = TILES * D;
   const AttnGeom& g = args.geom;
@@ -729,11 +785,22 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
   bool ok = true;
   RingPos2 spos, last_pv;     // TILES = 1: S buffers
   uint32_t blocks = 0, outs = 0;
+  uint32_t uses = 0;  // of the staging tile, by either tile
   if (TILES == 2) spos.slot = t;
   uint32_t taken = 0;
   FwdSeg s;
   while (fwd_take<true>(sh, taken, s, err, kErrWaitSoftmax, ok)) {
     const FwdTile tile = sh.work[taken & 1u].tile[t];
+    // tile 0's use of the staging tile comes before tile 1's
+    bool staged = false;
+    uint32_t use = 0;
+    if (TILES == 2) {
+      const bool s0 = fwd_staged<PAGED, STREAM>(g, s, sh.work[taken & 1u].tile[0]);
+      const bool s1 = fwd_staged<PAGED, STREAM>(g, s, sh.work[taken & 1u].tile[1]);
+      staged = t == 0 ? s0 : s1;
+      use = uses + (t == 1 && s0 ? 1u : 0u);
+      uses += (s0 ? 1u : 0u) + (s1 ? 1u : 0u);
+    }
     fwd_taken<true>(sh, taken);
     if (tile.t0 >= tile.t1) continue;
     const int token = tile.t0 + row_token;
@@ -873,25 +940,37 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
                  (static_cast<int64_t>(g.heads_kv) * g.g) + hd;
     };
     if (!STREAM || s.whole) {
-      if (live) {
-        const int64_t r = s.seq.row0 + token;
-        if (args.lse)
-          args.lse[lse_at(r, token, head)] =
-              l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
-        const float inv_l = l == 0.f ? 0.f : 1.0f / l;
-        T* orow = static_cast<T*>(args.out) + (PAGED ? 0 : s.b * args.o_batch) +
-                  r * args.o_token + head * args.o_head;
+      if (live && args.lse)
+        args.lse[lse_at(s.seq.row0 + token, token, head)] =
+            l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.6931471805599453f;
+      const float inv_l = l == 0.f ? 0.f : 1.0f / l;
+      T* orow = static_cast<T*>(args.out) + (PAGED ? 0 : s.b * args.o_batch) +
+                (s.seq.row0 + token) * args.o_token + head * args.o_head;
+      // the tile's last contents have been read out
+      if (staged && use > 0) {
+        ok = wait(&sh.stage_empty, (use - 1) & 1u);
+        if (!ok) break;
+      }
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t pk[8];
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t pk[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float lo = __uint_as_float(ov[c * 16 + 2 * e]) * inv_l;
-            const float hi = __uint_as_float(ov[c * 16 + 2 * e + 1]) * inv_l;
-            pk[e] = FMT == 1 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
-          }
+        for (int e = 0; e < 8; ++e) {
+          const float lo = __uint_as_float(ov[c * 16 + 2 * e]) * inv_l;
+          const float hi = __uint_as_float(ov[c * 16 + 2 * e + 1]) * inv_l;
+          pk[e] = FMT == 1 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+        }
+        if (staged) {
+          stage_chunk(stage, row, 2 * c, pk);
+          stage_chunk(stage, row, 2 * c + 1, pk + 4);
+        } else if (live) {
           store_pairs8(orow + c * 16, pk, args.wide);
         }
+      }
+      if (staged) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.stage_full));
       }
       continue;
     }
@@ -975,6 +1054,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q,
                     const __grid_constant__ CUtensorMap tma_k,
                     const __grid_constant__ CUtensorMap tma_v,
+                    const __grid_constant__ CUtensorMap tma_o,
                     const __grid_constant__ FwdArgs args) {
   using G = FwdGeom<D>;
   constexpr int NB = TILES == 1 ? kFwdSBufs : 2;
@@ -986,6 +1066,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
   const uint32_t q_smem = base;
   const uint32_t k_smem = q_smem + TILES * G::Q_BYTES;
   const uint32_t v_smem = k_smem + args.k_stages * G::KV_BYTES;
+  const uint32_t stage = v_smem + args.v_stages * G::KV_BYTES;  // TILES = 2
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -1012,12 +1093,15 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
       mbar_init(smem_u32(&sh.work_full[i]), 1);
       mbar_init(smem_u32(&sh.work_empty[i]), 3 + 4 * TILES);  // two producers, MMA, softmax warps
     }
+    mbar_init(smem_u32(&sh.stage_full), 4);
+    mbar_init(smem_u32(&sh.stage_empty), 1);
     mbar_init(smem_u32(&sh.drain), 1);
     sh.abort = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tma_q);
     tma_prefetch_desc(&tma_k);
     tma_prefetch_desc(&tma_v);
+    if (TILES == 2) tma_prefetch_desc(&tma_o);
   }
   if (warp == 2) {
     tmem_alloc(smem_u32(&sh.tmem_base), 512);
@@ -1042,10 +1126,10 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
     else if (warp == 1 && elect_one())
       fwd_mma<FMT, D, PAGED, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
     else if (warp == 2 && elect_one())
-      fwd_schedule<PAGED, STREAM, TILES>(args, sh);
+      fwd_schedule<D, PAGED, STREAM, TILES>(args, sh, &tma_o, stage);
   } else {
     if constexpr (TILES == 2) fwd_regs_inc<kFwdHighRegs>();
-    fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, tmem, warp, lane);
+    fwd_softmax<T, FMT, D, PAGED, STREAM, TILES>(args, sh, stage, tmem, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -1124,8 +1208,10 @@ uint64_t fwd_counter_bytes(const AttnGeom& g) {
 template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
 gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   const AttnGeom& g = p.geom;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
+  const HeadsView out{p.out, p.q.batch, p.q.tokens, p.q.heads, p.o_batch, p.o_token, p.o_head};
   if (!encode_rows_map(&mq, p.dtype, p.q, D, g.g, g.tpt) ||
+      !encode_rows_map(&mo, p.dtype, out, D, g.g, g.tpt) ||
       !encode_keys_map(&mk, p.dtype, p.k, D, g.box_rows) ||
       !encode_keys_map(&mv, p.dtype, p.v, D, g.box_rows))
     return GPO_BAD_ARGS;
@@ -1138,11 +1224,9 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   a.o_head = p.o_head;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.spans = fwd_spans(g);
-  // Two Q tiles of D = 128 leave room for five slots.  V gets three: PV of a
-  // block frees its slot one step before the slot's next block is needed, S
-  // of a block two steps before.
-  a.v_stages = kFwdMaxStages;
-  a.k_stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
+  // Two Q tiles and the staging tile of D = 128 leave room for four slots
+  // (a third V slot in the staging tile's place measured the same).
+  a.k_stages = a.v_stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
   a.wide = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0 && p.o_batch % 16 == 0 &&
            p.o_token % 16 == 0 && p.o_head % 16 == 0;
   a.err = c.err;
@@ -1160,11 +1244,12 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   }
   auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES>;
   const uint32_t dyn =
-      (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN) * D * 2u + 1024u;
+      (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN +
+       (TILES == 2 ? 128u : 0u)) * D * 2u + 1024u;
   gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
   return launch_in_order(kern, static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream, mq,
-                         mk, mv, a);
+                         mk, mv, mo, a);
 }
 
 template <typename T, int FMT, int D>

@@ -200,6 +200,43 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// 5-D tiled store of a swizzled tile in this CTA's shared memory.
+__device__ __forceinline__ void tma_store_5d(const CUtensorMap* map, uint32_t src, int32_t x,
+                                             int32_t y, int32_t z, int32_t u, int32_t v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5, %6}], "
+      "[%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int32_t x,
+                                             int32_t y, int32_t z, int32_t u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], "
+      "[%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's stores have read their shared memory / are done.
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// Eight 16-bit values (four pairs) of a row into a 128-byte-swizzled tile of
+// 128 rows: 16-byte chunk `c` (of 8 per 64 dims) of `row`.
+__device__ __forceinline__ void stage_chunk(uint32_t tile, int row, int c, const uint32_t* v) {
+  const uint32_t at = tile + (c / 8) * 128 * 128 + row * 128 + (((c % 8) ^ (row & 7)) << 4);
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
 // ------------------------------------------------------------------- host
 // One strided (batch, token, head, dim) tensor of 16-bit elements.
 struct HeadsView {
