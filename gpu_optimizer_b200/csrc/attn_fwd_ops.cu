@@ -1040,7 +1040,9 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
           if (c > c_last) ml.y = 0.f;
         };
         const int total = rows * (D / 4);
-        if (rows <= 16)
+        if (TILES == 1 && total > 128 && rows <= 16)
+          fwd_join<2, 8>(row, total, rows, c_first, c_last, part_row, finish);
+        else if (rows <= 16)
           fwd_join<1, 8>(row, total, rows, c_first, c_last, part_row, finish);
         else
           fwd_join<4, 2>(row, total, rows, c_first, c_last, part_row, finish);
