@@ -1182,8 +1182,12 @@ bool encode_keys_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, i
 
 namespace {
 
-// Two tiles per unit where a sequence can fill them.
-int fwd_tiles(const AttnGeom& g) { return g.q_len > g.tpt ? 2 : 1; }
+// Two tiles per unit where a sequence fills them and where there are more
+// tiles than SMs: with fewer, a tile per CTA ends earlier.
+int fwd_tiles(const AttnGeom& g) {
+  const int64_t tiles = static_cast<int64_t>(cdiv(g.q_len, g.tpt)) * g.batch * g.heads_kv;
+  return g.q_len > g.tpt && tiles > kFwdMaxCtas ? 2 : 1;
+}
 
 int fwd_spans(const AttnGeom& g) {
   return static_cast<int>(cdiv(static_cast<uint64_t>(g.q_len),
@@ -1268,7 +1272,8 @@ gpo_status run_fwd_form(const AttnProblem& p, const LaunchCtx& c) {
 }  // namespace
 
 uint64_t attn_paged_workspace(const AttnProblem& p) {
-  // whatever part of the plan's sequences and tokens a call has
+  // a call with part of the plan's sequences and tokens needs no more: its
+  // units have at most as many rows
   const AttnGeom& g = p.geom;
   return ((fwd_counter_bytes(g) + 255u) & ~255ull) +
          2u * kFwdMaxCtas * static_cast<uint64_t>(fwd_part_floats(fwd_part_rows(g), p.dim)) * 4u;

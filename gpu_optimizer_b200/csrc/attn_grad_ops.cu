@@ -85,8 +85,11 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
     const int r = r0 + lane / LPR;
     const int token = tile * g.tpt + r / g.g, head = h * g.g + r % g.g;
     const bool live = r < g.tpt * g.g && token < g.q_len;
-    float s = 0.f;
+    float s = 0.f, l = 0.f;
     if (live) {
+      if (lane % LPR == 0)
+        l = a.lse[(static_cast<int64_t>(b) * g.q_len + token) *
+                      (static_cast<int64_t>(g.heads_kv) * g.g) + head];
       const uint4 x = *reinterpret_cast<const uint4*>(
           static_cast<const T*>(a.out) + b * a.o_batch + token * a.o_token + head * a.o_head +
           (lane % LPR) * 8);
@@ -103,8 +106,6 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
     if (lane % LPR == 0) {
       float nl = -INFINITY;  // no query in this row: P is 0
       if (live) {
-        const float l = a.lse[(static_cast<int64_t>(b) * g.q_len + token) *
-                                  (static_cast<int64_t>(g.heads_kv) * g.g) + head];
         // a row that saw no key (L = -inf) has P = 0 everywhere, too
         nl = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
       }
