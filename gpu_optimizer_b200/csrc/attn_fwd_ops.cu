@@ -1185,8 +1185,10 @@ namespace {
 // Two tiles per unit where a sequence fills them and where there are more
 // tiles than SMs: with fewer, a tile per CTA ends earlier.
 int fwd_tiles(const AttnGeom& g) {
-  const int64_t tiles = static_cast<int64_t>(cdiv(g.q_len, g.tpt)) * g.batch * g.heads_kv;
-  return g.q_len > g.tpt && tiles > kFwdMaxCtas ? 2 : 1;
+  int64_t tiles = static_cast<int64_t>(cdiv(g.q_len, g.tpt)) * g.batch;
+  // paged: the rows of all sequences together fill no more than
+  if (g.kv_lens) tiles = std::min<int64_t>(tiles, g.tokens / g.tpt + g.batch);
+  return g.q_len > g.tpt && tiles * g.heads_kv > kFwdMaxCtas ? 2 : 1;
 }
 
 int fwd_spans(const AttnGeom& g) {
