@@ -22,7 +22,10 @@
 //   warp 3     TMA of the second own tile (V or dO) and of ring B (dO or V)
 //   warp 1     MMA issuer
 //   warp 2     TMEM owner; takes work items from a counter and works them out
-//   warps 4-11 elementwise: thread = TMEM lane, 64 of a tile's 128 columns
+//   warps 4-11  elementwise: thread = TMEM lane, 64 of a tile's 128 columns
+//   warps 12-15 read an item's sums out of TMEM and store them, while the
+//               elementwise warps go on with the next item (when they did it
+//               themselves, every item began some 4000 cycles later)
 // Ring A is three tiles deep and ring B two (with D = 128 that fills shared
 // memory): a tile of A is needed by the last product of a step and again
 // missing at the first product of the next but one, so with two slots the
@@ -34,9 +37,13 @@
 namespace gpo {
 
 constexpr int kGradA = 3, kGradB = 2;  // ring depths
-constexpr int kGradThreads = 384;      // 4 service warps, 2 x 4 elementwise warps
-constexpr int kGradEwWarps = 8;
-constexpr int kGradReaders = 3 + kGradEwWarps;  // of an item: producers, MMA, elementwise
+constexpr int kGradThreads = 512;      // 4 service, 8 elementwise, 4 storing warps
+constexpr int kGradEwWarps = 8, kGradOutWarps = 4;
+// 512 threads launch at 128 registers; an elementwise thread needs 168.
+constexpr int kGradLowRegs = 88, kGradEwRegs = 168, kGradOutRegs = 88;
+static_assert(128 * kGradLowRegs + 256 * kGradEwRegs + 128 * kGradOutRegs <= 128 * kGradThreads,
+              "register split exceeds the launch's registers");
+constexpr int kGradReaders = 3 + kGradEwWarps + kGradOutWarps;  // of an item: all but warp 2
 
 struct GradArgs {
   AttnGeom geom;
@@ -143,7 +150,7 @@ struct GradShared {
   uint64_t s_full[2], dp_full;       // key tiles use s_full[0] alone
   uint64_t q_s_full[2];              // the two S buffers of query tiles
   uint64_t p_ready, ds_ready;
-  uint64_t dv_full, acc_full, acc_free;
+  uint64_t sum_full[2], sum_free[2];  // dV; dK or dQ
   uint64_t item_full[2], item_empty[2];
   uint64_t drain;
   GradWork work[2];
@@ -180,9 +187,8 @@ __device__ __forceinline__ void grad_init(GradShared& sh) {
   init(sh.q_s_full, 2, 1);
   init(&sh.p_ready, 1, kGradEwWarps);
   init(&sh.ds_ready, 1, kGradEwWarps);
-  init(&sh.dv_full, 1, 1);
-  init(&sh.acc_full, 1, 1);
-  init(&sh.acc_free, 1, kGradEwWarps);
+  init(sh.sum_full, 2, 1);
+  init(sh.sum_free, 2, kGradOutWarps);
   init(sh.item_full, 2, 1);
   init(sh.item_empty, 2, kGradReaders);
   init(&sh.drain, 1, 1);
@@ -354,6 +360,15 @@ __device__ __forceinline__ void grad_schedule(const GradArgs& args, GradShared& 
   }
 }
 
+template <int N>
+__device__ __forceinline__ void grad_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void grad_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 struct GradMaps {
   const CUtensorMap *q, *dout, *k, *v;
 };
@@ -412,6 +427,20 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
     else
       load_rows(own_smem, SIDE == 0 ? maps.q : maps.dout, &sh.own_full[SIDE], qi.h, qi.t0, qi.b);
     ++own;
+    // the row statistics of a query tile, or of every query tile of a key tile
+    auto load_stats = [&](int b, int h, int tile) {
+      if (!wait(&sh.st_empty[st.slot], st.parity ^ 1u)) return false;
+      const uint32_t bar = smem_u32(&sh.st_full[st.slot]);
+      mbar_arrive_expect_tx(bar, 1024u);
+      bulk_load(base + G::STATS + st.slot * 1024u, grad_stats(args, b, h, tile), 1024u, bar);
+      ++stats;
+      st.step();
+      return true;
+    };
+    if (SIDE == 0 && !keys && !load_stats(qi.b, qi.h, qi.tile)) {
+      ok = false;
+      break;
+    }
     for (int j = 0; j < n; ++j) {
       if (!wait(&empty[pos.slot], pos.parity ^ 1u)) {
         ok = false;
@@ -426,17 +455,9 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
                   qi.b);
       ++issued;
       pos.step();
-      if (SIDE == 0 && keys) {
-        if (!wait(&sh.st_empty[st.slot], st.parity ^ 1u)) {
-          ok = false;
-          break;
-        }
-        const uint32_t bar = smem_u32(&sh.st_full[st.slot]);
-        mbar_arrive_expect_tx(bar, 1024u);
-        bulk_load(base + G::STATS + st.slot * 1024u, grad_stats(args, p.b, p.h, p.first + j),
-                  1024u, bar);
-        ++stats;
-        st.step();
+      if (SIDE == 0 && keys && !load_stats(p.b, p.h, p.first + j)) {
+        ok = false;
+        break;
       }
     }
     if (!ok) break;
@@ -491,7 +512,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
   bool ok = true, was_keys = true;
   GradRing<kGradA> a;  // next tile of ring A that has not been waited for
   GradRing<kGradB> b;
-  uint32_t own = 0, cnt = 0, qcnt = 0;
+  uint32_t own = 0, kown = 0, cnt = 0, qcnt = 0;
   uint32_t taken = 0;
   GradWork w;
   while (grad_take<false>(sh, taken, w, err, kErrWaitMma, ok)) {
@@ -510,17 +531,17 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
       mma_rows<D>(tmem + C::DP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
       commit(&sh.dp_full);
       if (n == 1) commit(&sh.own_empty[1]);
-      // the previous item's sums have been read out of TMEM
-      if (own > 0) ok = wait(&sh.acc_free, (own - 1) & 1u);
       for (int j = 0; j < n && ok; ++j, ++cnt) {
         const int aj = a.slot, bj = b.slot;
         const bool more = j + 1 < n;
         ok = wait(&sh.p_ready, cnt & 1u);
+        // the previous item's dV has been read out of TMEM
+        if (ok && j == 0 && own > 0) ok = wait(&sh.sum_free[0], (own - 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         mma_cols(tmem + C::DV, tmem + C::S, cols_of(G::RING_B, bj), IDESC_O, j == 0);
         commit(&sh.b_empty[bj]);
-        if (!more) commit(&sh.dv_full);
+        if (!more) commit(&sh.sum_full[0]);
         a.step();
         b.step();
         if (more) {
@@ -531,6 +552,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
           if (j + 2 == n) commit(&sh.own_empty[0]);
         }
         ok = wait(&sh.ds_ready, cnt & 1u);
+        if (ok && j == 0 && own > 0) ok = wait(&sh.sum_free[1], (own - 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         mma_cols(tmem + C::DK, tmem + C::DP, cols_of(G::RING_A, aj), IDESC_O, j == 0);
@@ -542,9 +564,10 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
           commit(&sh.dp_full);
           if (j + 2 == n) commit(&sh.own_empty[1]);
         } else {
-          commit(&sh.acc_full);
+          commit(&sh.sum_full[1]);
         }
       }
+      if (ok) ++kown;
     } else {
       ok = wait(&sh.own_full[0], op) && wait(&sh.a_full[a.slot], a.parity);
       if (!ok) break;
@@ -552,9 +575,10 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
       commit(&sh.q_s_full[qcnt & 1u]);
       if (n == 1) commit(&sh.own_empty[0]);
       ok = wait(&sh.own_full[1], op) && wait(&sh.b_full[b.slot], b.parity);
-      // dP of query tiles has the columns of dV of key tiles
-      const bool turn = was_keys && own > 0;
-      if (ok && turn) ok = wait(&sh.acc_free, (own - 1) & 1u);
+      // dP of query tiles has the columns of dV (and dK) of key tiles
+      const bool turn = was_keys && kown > 0;
+      if (ok && turn)
+        ok = wait(&sh.sum_free[0], (kown - 1) & 1u) && wait(&sh.sum_free[1], (own - 1) & 1u);
       if (!ok) break;
       was_keys = false;
       mma_rows<D>(tmem + C::QDP, own1, rows_of(G::RING_B, b.slot), IDESC_S);
@@ -562,7 +586,6 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
       commit(&sh.b_empty[b.slot]);
       b.step();
       if (n == 1) commit(&sh.own_empty[1]);
-      if (own > 0 && !turn) ok = wait(&sh.acc_free, (own - 1) & 1u);
       for (int j = 0; j < n && ok; ++j, ++cnt, ++qcnt) {
         const int aj = a.slot;
         const bool more = j + 1 < n;
@@ -587,10 +610,16 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
           b.step();
           if (j + 2 == n) commit(&sh.own_empty[1]);
         }
+        // the previous item's dQ has been read out of TMEM
+        if (j == 0 && own > 0 && !turn) {
+          ok = wait(&sh.sum_free[1], (own - 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+        }
         mma_cols(tmem + C::DQ, tmem + C::QS + (qcnt & 1u) * 128, cols_of(G::RING_A, aj), IDESC_O,
                  j == 0);
         commit(&sh.a_empty[aj]);
-        if (!more) commit(&sh.acc_full);
+        if (!more) commit(&sh.sum_full[1]);
       }
     }
     if (!ok) break;
@@ -612,7 +641,7 @@ struct GradEw {
   uint32_t lane_addr;
   bool ok = true;
   GradRing<2> st;
-  uint32_t own = 0, kown = 0, cnt = 0, qcnt = 0;  // items, key tiles; steps, of query tiles
+  uint32_t cnt = 0, qcnt = 0;  // steps, steps of query tiles
 
   __device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity) {
     return ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &sh.abort, args.err,
@@ -654,13 +683,6 @@ struct GradEw {
     const float2 s = __fmul2_rn(make_float2(pr[i], pr[i + 1]), d);
     return pack2<FMT>(s.x, s.y);
   }
-  __device__ __forceinline__ void acc_release() {
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sh.acc_free));
-    ++own;
-  }
-
   // thread = key; 64 packed query rows of the tile
   __device__ __forceinline__ void keys(const KvPiece& p) {
     using G = GradGeom<D>;
@@ -747,47 +769,6 @@ struct GradEw {
       if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
       st.step();
     }
-    // dV first, while the last dK product still runs; each warpgroup has
-    // half of the dims
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      if (p.n > 0) {
-        if (!wait(m == 0 ? &sh.dv_full : &sh.acc_full, (m == 0 ? kown : own) & 1u)) return;
-        tc_fence_after();
-      }
-      constexpr int H = D / 2;
-      const uint32_t acc = tmem + lane_addr + (m == 0 ? C::DV : C::DK) + wg * H;
-      const float f = m == 0 ? 1.f : args.scale;
-      const bool sink = key < g.sinks;
-      if (k0 < g.sinks) {
-        float* part =
-            sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + m * D + wg * H : nullptr;
-#pragma unroll 1
-        for (int c = 0; c < H / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(acc + c * 32, r);
-          tmem_wait_ld();
-          if (sink && key < g.kv_len) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + c * 32 + i) =
-                  p.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                           : make_float4(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f,
-                                         __uint_as_float(r[i + 2]) * f,
-                                         __uint_as_float(r[i + 3]) * f);
-          }
-        }
-      }
-      T* dst = m == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
-                            p.h * args.dv_head
-                      : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
-                            p.h * args.dk_head;
-      if (p.piece == 0)
-        store_row<T, FMT, H>(acc, dst + wg * H, f, key < g.kv_len && !sink, p.n == 0,
-                             args.wide_dkv);
-    }
-    if (p.n > 0) ++kown;
-    if (p.n > 0) acc_release();
   }
 
   // thread = packed query row; 64 keys of the block
@@ -796,11 +777,18 @@ struct GradEw {
     const AttnGeom& g = args.geom;
     const uint32_t dp_t = tmem + lane_addr + C::QDP + wg * 64;
     const float2 scale2 = make_float2(args.scale_log2, args.scale_log2);
-    const int row_token = row / g.g, row_head = row % g.g;
-    const int token = it.t0 + row_token;
-    const bool live = row_token < g.tpt && token < it.t1;
-    const float* stat = grad_stats(args, it.b, it.h, it.tile);
-    const float nl = stat[row], nd = stat[128 + row];
+    const int token = it.t0 + row / g.g;
+    if (it.blk.n == 0) return;
+    if (!wait(&sh.st_full[st.slot], st.parity)) return;
+    float nl, nd;
+    {
+      const uint32_t stat = base + GradGeom<D>::STATS + st.slot * 1024u + row * 4;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(nl) : "r"(stat));
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(nd) : "r"(stat + 512));
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
+    st.step();
     const float2 shift2 = make_float2(nl, nl), delta2 = make_float2(nd, nd);
     for (int j = 0; j < it.blk.n; ++j, ++cnt, ++qcnt) {
       const int key0 = it.blk.at(j) * 128;
@@ -837,18 +825,84 @@ struct GradEw {
       tmem_st32(s_t, pk);
       release(&sh.ds_ready);
     }
-    if (it.blk.n > 0) {
-      if (!wait(&sh.acc_full, own & 1u)) return;
-      tc_fence_after();
-    }
-    // each warpgroup writes half of the dims
-    T* dst = static_cast<T*>(args.dq) + it.b * args.dq_batch + token * args.dq_token +
-             (it.h * g.g + row_head) * args.dq_head + wg * (D / 2);
-    store_row<T, FMT, D / 2>(tmem + lane_addr + C::DQ + wg * (D / 2), dst, args.scale, live,
-                             it.blk.n == 0, args.wide_dq);
-    if (it.blk.n > 0) acc_release();
   }
 };
+
+// ---------------------------------------------------------- sums to memory
+// Thread = TMEM lane: a key's dV and dK, or a query row's dQ.
+template <typename T, int FMT, int D>
+__device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, uint32_t tmem,
+                                         int quarter, int lane) {
+  using C = GradTmem<D>;
+  const AttnGeom& g = args.geom;
+  const int row = quarter * 32 + lane;
+  const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+  const int row_token = row / g.g, row_head = row % g.g;
+  bool ok = true;
+  uint32_t taken = 0, own = 0, kown = 0;
+  auto wait = [&](const uint64_t* bar, uint32_t parity) {
+    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, &sh.abort, args.err,
+                                           kErrWaitEpilogue));
+    if (ok) tc_fence_after();
+    return ok;
+  };
+  auto release = [&](uint64_t* bar) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(bar));
+  };
+  GradWork w;
+  while (grad_take<true>(sh, taken, w, args.err, kErrWaitEpilogue, ok)) {
+    if (w.kind == 1) {
+      const KvPiece& p = w.p;
+      const int key = p.kt * 128 + row;
+      const bool there = key < g.kv_len, sink = key < g.sinks;
+#pragma unroll 1
+      for (int m = 0; m < 2; ++m) {
+        if (w.n > 0 && !wait(&sh.sum_full[m], (m == 0 ? kown : own) & 1u)) return;
+        const uint32_t acc = tmem + lane_addr + (m == 0 ? C::DV : C::DK);
+        const float f = m == 0 ? 1.f : args.scale;
+        if (p.kt * 128 < g.sinks) {
+          float* part = sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + m * D : nullptr;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(acc + c * 32, r);
+            tmem_wait_ld();
+            if (sink && there) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part + c * 32 + i) =
+                    w.n == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                             : make_float4(__uint_as_float(r[i]) * f,
+                                           __uint_as_float(r[i + 1]) * f,
+                                           __uint_as_float(r[i + 2]) * f,
+                                           __uint_as_float(r[i + 3]) * f);
+            }
+          }
+        }
+        T* dst = m == 0 ? static_cast<T*>(args.dv) + p.b * args.dv_batch + key * args.dv_token +
+                              p.h * args.dv_head
+                        : static_cast<T*>(args.dk) + p.b * args.dk_batch + key * args.dk_token +
+                              p.h * args.dk_head;
+        if (p.piece == 0)
+          store_row<T, FMT, D>(acc, dst, f, there && !sink, w.n == 0, args.wide_dkv);
+        if (w.n > 0) release(&sh.sum_free[m]);
+      }
+      if (w.n > 0) ++kown;
+    } else {
+      const QItem& it = w.q;
+      const int token = it.t0 + row_token;
+      if (w.n > 0 && !wait(&sh.sum_full[1], own & 1u)) return;
+      T* dst = static_cast<T*>(args.dq) + it.b * args.dq_batch + token * args.dq_token +
+               (it.h * g.g + row_head) * args.dq_head;
+      store_row<T, FMT, D>(tmem + lane_addr + C::DQ, dst, args.scale,
+                           row_token < g.tpt && token < it.t1, w.n == 0, args.wide_dq);
+      if (w.n > 0) release(&sh.sum_free[1]);
+    }
+    if (w.n > 0) ++own;
+  }
+}
 
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(kGradThreads, 1)
@@ -902,15 +956,19 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   const uint32_t tmem = sh.tmem_base;
   let_next_start();
   wait_for_previous();
-  if (warp == 0) {
-    if (elect_one()) grad_producer<D, 0>(args, sh, maps, base);
-  } else if (warp == 3) {
-    if (elect_one()) grad_producer<D, 1>(args, sh, maps, base);
-  } else if (warp == 1) {
-    if (elect_one()) grad_mma<FMT, D>(args, sh, base, tmem);
-  } else if (warp == 2) {
-    if (elect_one()) grad_schedule(args, sh);
-  } else if (warp >= 4) {
+  if (warp < 4) {
+    grad_regs_dec<kGradLowRegs>();
+    if (warp == 0) {
+      if (elect_one()) grad_producer<D, 0>(args, sh, maps, base);
+    } else if (warp == 1) {
+      if (elect_one()) grad_mma<FMT, D>(args, sh, base, tmem);
+    } else if (warp == 2) {
+      if (elect_one()) grad_schedule(args, sh);
+    } else {
+      if (elect_one()) grad_producer<D, 1>(args, sh, maps, base);
+    }
+  } else if (warp < 12) {
+    grad_regs_inc<kGradEwRegs>();
     const int q = warp & 3;
     GradEw<T, FMT, D> ew{args, sh, base, tmem, (warp - 4) >> 2, q * 32 + lane, lane,
                          static_cast<uint32_t>(q * 32) << 16};
@@ -923,6 +981,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         ew.rows(w.q);
       if (!ew.ok) break;
     }
+  } else {
+    grad_regs_dec<kGradOutRegs>();
+    grad_out<T, FMT, D>(args, sh, tmem, warp & 3, lane);
   }
   tc_fence_before();
   __syncthreads();
