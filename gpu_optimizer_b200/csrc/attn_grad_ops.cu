@@ -683,6 +683,11 @@ struct GradEw {
     const float2 s = __fmul2_rn(make_float2(pr[i], pr[i + 1]), d);
     return pack2<FMT>(s.x, s.y);
   }
+  static __device__ __forceinline__ void mask_pairs(uint32_t (&pk)[32], const uint32_t (&see)[2]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) pk[i] &= pair_mask(see[i / 16], i % 16);
+  }
+
   // thread = key; 64 packed query rows of the tile
   __device__ __forceinline__ void keys(const KvPiece& p) {
     using G = GradGeom<D>;
@@ -706,7 +711,26 @@ struct GradEw {
       // packed rows of this thread's half that see the key: [c_lo, c_hi)
       const int c_lo = (max(tok_lo, ta) - ta) * g.g - wg * 64;
       const int c_hi = (min(tok_hi, tb) - ta + 1) * g.g - wg * 64;
+      const uint32_t see[2] = {bits_below(c_hi, 0) & ~bits_below(c_lo, 0),
+                               bits_below(c_hi, 1) & ~bits_below(c_lo, 1)};
       if (!wait(&sh.st_full[st.slot], st.parity) || !wait(&sh.s_full[0], cnt & 1u)) return;
+      if (masked && __all_sync(0xffffffffu, (see[0] | see[1]) == 0u)) {
+        // no key of this warp is seen by its rows (behind the window of a
+        // tile whose sinks are): P and dS are 0
+        uint32_t zero[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) zero[i] = 0u;
+        tc_fence_after();
+        tmem_st32(s_t, zero);
+        release(&sh.p_ready);
+        if (!wait(&sh.dp_full, cnt & 1u)) return;
+        tc_fence_after();
+        tmem_st32(dp_t, zero);
+        release(&sh.ds_ready);
+        if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
+        st.step();
+        continue;
+      }
       tc_fence_after();
       const uint32_t stat = base + G::STATS + st.slot * 1024u + wg * 256;
       float pr[64];
@@ -722,18 +746,12 @@ struct GradEw {
         exp2_to(pr, i + 2, __ffma2_rn(make_float2(pr[i + 2], pr[i + 3]), scale2,
                                       make_float2(nl.z, nl.w)));
       }
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t see = bits_below(c_hi, c) & ~bits_below(c_lo, c);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pr[c * 32 + i] = (see & (1u << i)) ? pr[c * 32 + i] : 0.f;
-        }
-      }
       {
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) pk[i] = pack2<FMT>(pr[2 * i], pr[2 * i + 1]);
+        // masked after packing (two values per operation, whatever they are)
+        if (masked) mask_pairs(pk, see);
         tmem_st32(s_t, pk);
       }
       release(&sh.p_ready);
@@ -755,15 +773,7 @@ struct GradEw {
           pk[c * 16 + i / 2 + 1] = ds_pair(pr, c * 32 + i + 2, dp, i + 2, make_float2(dl.z, dl.w));
         }
       }
-      if (masked) {
-        // 0 * (dP - delta) is not 0 when the masked dP is not finite
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint32_t see = (bits_below(c_hi, i / 16) & ~bits_below(c_lo, i / 16)) >>
-                               (2 * (i % 16));
-          pk[i] &= ((see & 1u) ? 0x0000ffffu : 0u) | ((see & 2u) ? 0xffff0000u : 0u);
-        }
-      }
+      if (masked) mask_pairs(pk, see);
       tmem_st32(dp_t, pk);
       release(&sh.ds_ready);
       if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st.slot]));
@@ -814,13 +824,10 @@ struct GradEw {
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
           pk[c * 16 + i / 2] = ds_pair(pr, c * 32 + i, dp, i, delta2);
-        if (masked) {
-          const uint32_t see = rm.word(c);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            pk[c * 16 + i] &= ((see & (1u << (2 * i))) ? 0x0000ffffu : 0u) |
-                              ((see & (2u << (2 * i))) ? 0xffff0000u : 0u);
-        }
+      }
+      if (masked) {
+        const uint32_t see[2] = {rm.word(0), rm.word(1)};
+        mask_pairs(pk, see);
       }
       tmem_st32(s_t, pk);
       release(&sh.ds_ready);

@@ -96,6 +96,22 @@ __device__ __forceinline__ uint32_t bits_below(int n, int c) {
   return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
 }
 
+// Mask of a packed 16-bit pair: 0xffff in each half whose bit (2 i, 2 i + 1)
+// of `see` is set.  The bit is shifted to the top of its byte and replicated
+// from there by the byte permutation's sign mode; the eight shifts are shared
+// by the 16 pairs of a word.
+__device__ __forceinline__ uint32_t pair_mask(uint32_t see, int i) {
+  const int lo = 2 * i, hi = 2 * i + 1;
+  const uint32_t a = see << (7 - (lo & 7)), b = see << (7 - (hi & 7));
+  const uint32_t from_a = 8u | static_cast<uint32_t>(lo >> 3);
+  const uint32_t from_b = 8u | 4u | static_cast<uint32_t>(hi >> 3);
+  uint32_t m;
+  asm("prmt.b32 %0, %1, %2, %3;"
+      : "=r"(m)
+      : "r"(a), "r"(b), "r"(from_a | from_a << 4 | from_b << 8 | from_b << 12));
+  return m;
+}
+
 // Keys of a block that a row at position p sees: i <= p - key0 and
 // (i > p - key0 - window or i < sinks - key0), i counted from the block's
 // first key; as mask words, which cost a test and a select per score.
