@@ -92,7 +92,10 @@ struct FwdShared {
   uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared behind the last key
   uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], p_half[2], pv_done[kFwdSBufs];
   uint64_t o_full[2], o_free[2];
-  uint64_t stage_full, stage_empty;  // one staging tile for both tiles of O
+  // One staging tile for both tiles of O.  Use u has been stored when phase
+  // u / 4 of stage_empty[u % 4] is done: a warpgroup without blocks can be two
+  // units ahead of the other, more than one barrier's two phases can tell.
+  uint64_t stage_full, stage_empty[4];
   int stage_at[8][3];                // batch, head, first row of the coming uses
   uint64_t drain;
   // cut launches: where this CTA's stretch begins
@@ -277,7 +280,7 @@ __device__ __forceinline__ void fwd_schedule(const FwdArgs& args, FwdShared& sh,
         tma_store_5d(tma_o, stage + c * 128 * 128, c * 64, 0, at[1], at[2], at[0]);
       bulk_commit();
       bulk_wait_read();
-      mbar_arrive(smem_u32(&sh.stage_empty));
+      mbar_arrive(smem_u32(&sh.stage_empty[stored & 3]));
       ++stored;
       moved = true;
     }
@@ -948,7 +951,7 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
                 (s.seq.row0 + token) * args.o_token + head * args.o_head;
       // the tile's last contents have been read out
       if (staged && use > 0) {
-        ok = wait(&sh.stage_empty, (use - 1) & 1u);
+        ok = wait(&sh.stage_empty[(use - 1) & 3], ((use - 1) >> 2) & 1u);
         if (!ok) break;
       }
 #pragma unroll
@@ -1096,7 +1099,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
       mbar_init(smem_u32(&sh.work_empty[i]), 3 + 4 * TILES);  // two producers, MMA, softmax warps
     }
     mbar_init(smem_u32(&sh.stage_full), 4);
-    mbar_init(smem_u32(&sh.stage_empty), 1);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&sh.stage_empty[i]), 1);
     mbar_init(smem_u32(&sh.drain), 1);
     sh.abort = 0;
     fence_barrier_init();
