@@ -83,6 +83,7 @@ class _WindowAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         return (*window_attention_backward(dout, *ctx.saved_tensors, **ctx.mask), None, None, None)
 
