@@ -23,6 +23,9 @@ head_dim 64 or 128.  Any strides whose rows of head_dim are contiguous and
 16-byte aligned are read in place (slices of a fused projection, transposed
 views); others are copied first.
 
+P and dS enter the tensor cores in the inputs' type (every sum is fp32).  With
+float16, dS below 2^-24 vanishes: scale the loss, as for any float16 training.
+
 Everything runs on torch's current stream and never synchronises.  A refused
 argument raises ``KernelBuildError`` with the library's reason, before
 anything is launched; a launch that fails raises ``RuntimeError``.

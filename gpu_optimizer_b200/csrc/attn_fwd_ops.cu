@@ -1047,8 +1047,60 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
           fwd_join<2, 8>(row, total, rows, c_first, c_last, part_row, finish);
         else if (rows <= 16)
           fwd_join<1, 8>(row, total, rows, c_first, c_last, part_row, finish);
-        else
-          fwd_join<4, 2>(row, total, rows, c_first, c_last, part_row, finish);
+        else if (row < rows) {
+          // thread = row: its weights first, then 32 dims of two parts at a
+          // time (16 loads in flight), which leave as 32-byte stores
+          float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            const float2 ml = __ldcg(part_ml(part_of(c)) + base + row);
+            if (ml.y != 0.f) {
+              const float to = fmaxf(m, ml.x);
+              sum = sum * ex2_approx(m - to) + ml.y * ex2_approx(ml.x - to);
+              m = to;
+            }
+          }
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          const int64_t at = s.seq.row0 + token;
+          if (args.lse)
+            args.lse[lse_at(at, token, head)] =
+                sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+          T* orow = static_cast<T*>(args.out) + at * args.o_token + head * args.o_head;
+#pragma unroll 1
+          for (int x0 = 0; x0 < D / 4; x0 += 8) {
+            float4 o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int c = c_first; c <= c_last; ++c) {
+              float* part = part_of(c);
+              const float2 ml = __ldcg(part_ml(part) + base + row);
+              float4 v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                v[i] = __ldcg(reinterpret_cast<const float4*>(part) + base + row +
+                              (x0 + i) * args.part_rows);
+              if (ml.y != 0.f) {  // a part without a key says nothing
+                const float f = ex2_approx(ml.x - m) * inv;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[i].x += v[i].x * f;
+                  o[i].y += v[i].y * f;
+                  o[i].z += v[i].z * f;
+                  o[i].w += v[i].w * f;
+                }
+              }
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              pk[2 * i] = FMT == 1 ? pack_bf16(o[i].x, o[i].y) : pack_f16(o[i].x, o[i].y);
+              pk[2 * i + 1] = FMT == 1 ? pack_bf16(o[i].z, o[i].w) : pack_f16(o[i].z, o[i].w);
+            }
+            store_pairs8(orow + x0 * 4, pk, args.wide);
+            store_pairs8(orow + x0 * 4 + 16, pk + 8, args.wide);
+          }
+        }
       }
     }
   }

@@ -277,7 +277,9 @@ typedef struct gpo_paged_args {
 GPO_API gpo_status gpo_window_attention(const gpo_window_args* args, void* stream, char* log,
                                         size_t log_cap);
 /* Gradients dq, dk, dv from dout, the inputs and the forward's out and lse.
- * Sums are taken in a fixed order: equal inputs give equal bits. */
+ * Sums are taken in a fixed order: equal inputs give equal bits.  P and dS
+ * are rounded to `dtype` between the products (GPO_FLOAT16: dS below 2^-24
+ * vanishes; scale the loss). */
 GPO_API gpo_status gpo_window_attention_grad(const gpo_window_args* args, void* stream, char* log,
                                              size_t log_cap);
 /* Bytes of workspace that gpo_window_attention_grad needs for `args` (its
