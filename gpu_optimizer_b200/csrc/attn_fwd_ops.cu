@@ -15,10 +15,11 @@
 //              staged tiles of O to memory
 //   warps 4-7  softmax and epilogue of tile 0, thread = query row = TMEM
 //   warps 8-11 lane; of tile 1
-// TILES = 2 (more than 128 rows per sequence and kv head): both tiles share
-// every K/V block; the issuer alternates them, so that one tile's softmax
-// hides behind the other's MMAs.  TILES = 1 (single tokens, short chunks):
-// bound by the K/V bytes; three S buffers let S run two blocks ahead of PV.
+// TILES = 2 (more than 128 rows per sequence and kv head, more than two tiles
+// per SM): both tiles share every K/V block; the issuer alternates them, so
+// that one tile's softmax hides behind the other's MMAs.  TILES = 1 (single
+// tokens, short chunks): bound by the K/V bytes; three S buffers let S run two
+// blocks ahead of PV.
 //
 // With TILES = 2 a whole tile of O leaves through a staging tile in shared
 // memory and TMA.  (Stores straight from the rows' threads touch 32 lines
@@ -30,13 +31,29 @@
 // for outside the tensor, which TMA fills with zeros.
 //
 // Whole units (many of them) are dealt out in rounds, the longest rows first
-// and every other round backwards.  Few units (STREAM, paged only) are cut: all units' blocks form one
-// line, and every CTA takes an equal stretch of it, whatever the lengths of
-// the sequences, which only the device knows (or an equal number of whole
-// units, where that takes no longer).  A unit that lies in one
-// stretch is finished by its CTA; of one that is cut, every CTA writes its
-// part (O unnormalised, maximum, sum) to the workspace and the CTA that
-// arrives last joins the parts in their order.
+// and every other round backwards.  Few units (STREAM, paged only) are cut:
+// all units' blocks form one line, and every CTA takes an equal stretch of it,
+// whatever the lengths of the sequences, which only the device knows (or an
+// equal number of whole units, where that takes no longer).  A unit that lies
+// in one stretch is finished by its CTA; of one that is cut, every CTA writes
+// its part (O unnormalised, maximum, sum) to the workspace and the CTA that
+// arrives last joins the parts in their order, at once: left to the end of
+// the CTAs' work, the joins met there (16 chunks of 512 over 2K: 231 -> 249 us).
+//
+// What bounds it, bf16, D 128, 32 heads over 8 (B200, 6.55 TB/s and 1650
+// TFLOP/s measured):
+//   prefill of 8192, window 1024   155 us, 834 TFLOP/s of the visible pairs;
+//                                  the tensor pipe and the exp2 unit are both
+//                                  busy 53 % of the time: a step of a pair of
+//                                  tiles (2.1 us) is the chain S -> maximum ->
+//                                  exp2 -> P -> PV, twice, half overlapped
+//   4 x 4096 causal                495 us, 1110 TFLOP/s, as above
+//   64 single tokens, 0.8K..8K     191 us, 0.91 of the copy rate: HBM
+//   2 single tokens, 4 kv heads,   98 us, 0.83 of it: HBM, and SMs that end up
+//     128K                         to a third before the last
+//   one token over 777             11 us: launch, a chain of dependent loads
+//                                  (length, page, K, V) and the join
+//   4 chunks of 512 over 8K        231 us, 1030 TFLOP/s; as the prefill
 #include <algorithm>
 
 #include "attn_ops.cuh"
@@ -47,7 +64,10 @@ constexpr int kFwdMaxStages = 3;       // slots of the K ring and of the V ring
 constexpr int kFwdSBufs = 3;           // S/P buffers (TILES = 1)
 constexpr float kFwdRescale = 8.0f;    // see the softmax
 constexpr int kFwdMaxCtas = 160;       // CTAs that a workspace has room for
-constexpr int kFwdCutCost = 5;         // blocks' time that writing and joining parts takes
+// Blocks' time that writing and joining parts takes.  0, 2, 5, 12, window
+// 1024: 4 chunks of 512 over 8K 83.4, 83.5, 59.2, 59.1 us; 12 chunks of up to
+// 300 over 6K 31.7, 20.3, 20.2, 20.2.
+constexpr int kFwdCutCost = 5;
 constexpr int kFwdStreamPairs = 1024;  // most (sequence, span) pairs of a cut launch
 // Registers of TILES = 2: 384 threads launch at 168; 128 * 88 + 256 * 208 is
 // the same total (a softmax thread holds a row of 128 scores).
@@ -1237,13 +1257,16 @@ bool encode_keys_map(CUtensorMap* map, int dtype, const HeadsView& t, int dim, i
 
 namespace {
 
-// Two tiles per unit where a sequence fills them and where there are more
-// tiles than SMs: with fewer, a tile per CTA ends earlier.
+// Two tiles per unit where a sequence fills them and where every SM gets
+// more than two tiles: with fewer, a tile per CTA ends earlier.  One tile
+// against two, bf16, D 128, 32 heads over 8, window 1024: 1 x 512 tokens
+// 10.6 / 14.4 us, 1024 17.3 / 22.6, 2048 43.5 / 41.5, 8192 183 / 155; paged,
+// 4 chunks of 512 over 8K 293 / 247.
 int fwd_tiles(const AttnGeom& g) {
   int64_t tiles = static_cast<int64_t>(cdiv(g.q_len, g.tpt)) * g.batch;
   // paged: the rows of all sequences together fill no more than
   if (g.kv_lens) tiles = std::min<int64_t>(tiles, g.tokens / g.tpt + g.batch);
-  return g.q_len > g.tpt && tiles * g.heads_kv > kFwdMaxCtas ? 2 : 1;
+  return g.q_len > g.tpt && tiles * g.heads_kv > 2 * kFwdMaxCtas ? 2 : 1;
 }
 
 int fwd_spans(const AttnGeom& g) {
@@ -1252,7 +1275,13 @@ int fwd_spans(const AttnGeom& g) {
 }
 
 // Units are cut where whole ones would leave SMs idle in the last round:
-// fewer than eight rounds of them.
+// fewer than eight rounds of them.  Cut against whole (us): single tokens
+// over 2 x 128K 98 / 1097, over 64 x 0.8K..8K 191 / 232; chunks of up to 300
+// over 12 x 1.2K..6K, window 1024, 20.2 / 40.2; 4 chunks of 512 over 8K
+// 231 / 237.  Where lengths happen to fill the rounds, whole units would win
+// (single tokens over 128 x 2K 116 / 109, 16 chunks of 512 over 2K 231 / 206),
+// but the lengths are on the device: cutting loses 12 % at most, whole units
+// lose any factor.
 bool fwd_is_cut(const AttnGeom& g) {
   const int64_t pairs = static_cast<int64_t>(fwd_spans(g)) * g.batch;
   return pairs <= kFwdStreamPairs && pairs * g.heads_kv < 8 * kFwdMaxCtas;

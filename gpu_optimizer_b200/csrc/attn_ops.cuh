@@ -164,6 +164,8 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 
 // Eight 16-bit pairs to global memory: one 32-byte store where the address
 // allows (a row per lane: a whole sector per lane and half the wavefronts).
+// Gradients of 8192 tokens whose rows start on 32 bytes against 16: 447..460
+// us and 452..465.
 __device__ __forceinline__ void store_pairs8(void* dst, const uint32_t* v, bool wide) {
   if (wide) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]),
