@@ -448,51 +448,54 @@ __device__ __forceinline__ void fwd_barrier(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
-// Joins the parts [c0, c1] of a unit's elements (of which this thread has
-// every 128th), in their order and against a running maximum.  U elements
-// times P parts are loaded before the first is used: the loop is bound by
-// the latency of these loads.
-template <int U, int P, typename Load, typename Finish>
-__device__ __forceinline__ void fwd_join(int first, int total, int rows, int c0, int c1,
-                                         Load&& load, Finish&& finish) {
-  for (int e0 = first; e0 < total; e0 += 128 * U) {
-    float4 o[U];
-    float m[U], sum[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      m[u] = -INFINITY;
-      sum[u] = 0.f;
-    }
+// Joins the parts [c0, c1] of a unit with few rows (16 at most), in their
+// order and against a running maximum.  A thread has every nx-th vector of four
+// dims of one row; those of 16 parts are loaded before the first is used, as
+// the loop is bound by the latency of these loads (one token over 8K: 15.2 us,
+// with 8 parts of two vectors 16.2; 16 parts of two spill).
+template <typename LoadMl, typename Load, typename Finish>
+__device__ __forceinline__ void fwd_join(int id, int rows, int vecs, int c0, int c1,
+                                         LoadMl&& load_ml, Load&& load, Finish&& finish) {
+  constexpr int P = 16;
+  const int nx = 128 / rows, r = id % rows;
+  if (id / rows >= nx) return;
+  for (int x = id / rows; x < vecs; x += nx) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll 1
     for (int c = c0; c <= c1; c += P) {
-      float2 ml[U][P];
-      float4 v[U][P];
+      float2 ml[P];
+      float4 v[P];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int e = min(e0 + u * 128, total - 1);
-#pragma unroll
-        for (int i = 0; i < P; ++i) load(c + i, e % rows, e / rows, ml[u][i], v[u][i]);
+      for (int i = 0; i < P; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        if (c + i <= c1) {
+          ml[i] = load_ml(c + i, r);
+          v[i] = load(c + i, r, x);
+        }
       }
+      float top = m;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < P; ++i) top = fmaxf(top, ml[i].y != 0.f ? ml[i].x : -INFINITY);
+      const float a = m == top ? 1.f : ex2_approx(m - top);
+      m = top;
+      sum *= a;
+      o.x *= a;
+      o.y *= a;
+      o.z *= a;
+      o.w *= a;
 #pragma unroll
-        for (int i = 0; i < P; ++i)
-          if (ml[u][i].y != 0.f) {  // a part without a key says nothing
-            const float to = fmaxf(m[u], ml[u][i].x);
-            const float a = ex2_approx(m[u] - to), f = ex2_approx(ml[u][i].x - to);
-            m[u] = to;
-            sum[u] = sum[u] * a + ml[u][i].y * f;
-            o[u].x = o[u].x * a + v[u][i].x * f;
-            o[u].y = o[u].y * a + v[u][i].y * f;
-            o[u].z = o[u].z * a + v[u][i].z * f;
-            o[u].w = o[u].w * a + v[u][i].w * f;
-          }
+      for (int i = 0; i < P; ++i)
+        if (ml[i].y != 0.f) {  // a part without a key says nothing
+          const float f = ex2_approx(ml[i].x - top);
+          sum += ml[i].y * f;
+          o.x += v[i].x * f;
+          o.y += v[i].y * f;
+          o.z += v[i].z * f;
+          o.w += v[i].w * f;
+        }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * 128;
-      if (e < total) finish(e % rows, e / rows, o[u], m[u], sum[u]);
-    }
+    finish(r, x, o, m, sum);
   }
 }
 
@@ -1056,18 +1059,14 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
                                        : pack_f16(o.z * inv, o.w * inv);
           reinterpret_cast<uint2*>(orow)[x] = make_uint2(lo, hi);
         };
-        auto part_row = [&](int c, int r, int x, float2& ml, float4& v) {
-          float* part = part_of(min(c, c_last));
-          ml = __ldcg(part_ml(part) + base + r);
-          v = __ldcg(reinterpret_cast<const float4*>(part) + base + r + x * args.part_rows);
-          if (c > c_last) ml.y = 0.f;
+        auto load_ml = [&](int c, int r) { return __ldcg(part_ml(part_of(c)) + base + r); };
+        auto load = [&](int c, int r, int x) {
+          return __ldcg(reinterpret_cast<const float4*>(part_of(c)) + base + r +
+                        x * args.part_rows);
         };
-        const int total = rows * (D / 4);
-        if (TILES == 1 && total > 128 && rows <= 16)
-          fwd_join<2, 8>(row, total, rows, c_first, c_last, part_row, finish);
-        else if (rows <= 16)
-          fwd_join<1, 8>(row, total, rows, c_first, c_last, part_row, finish);
-        else if (row < rows) {
+        if (rows <= 16) {
+          fwd_join(row, rows, D / 4, c_first, c_last, load_ml, load, finish);
+        } else if (row < rows) {
           // thread = row: its weights first, then 32 dims of two parts at a
           // time (16 loads in flight), which leave as 32-byte stores
           float m = -INFINITY, sum = 0.f;
