@@ -59,7 +59,7 @@ struct GradArgs {
   int64_t dq_batch, dq_token, dq_head, dk_batch, dk_token, dk_head, dv_batch, dv_token, dv_head;
   float scale, scale_log2;
   int kv_tiles;    // key tiles of a head
-  int sink_tiles;  // of them, tiles with a sink key
+  int sink_tiles;  // of them, tiles with a sink key; 0: nothing to join
   int far_tiles;   // query tiles of a far piece (see kv_piece)
   int far_pieces;  // far pieces of a sink tile
   int kv_items, items;     // items [0, kv_items): key tiles, then query tiles
@@ -863,13 +863,13 @@ __device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, u
     if (w.kind == 1) {
       const KvPiece& p = w.p;
       const int key = p.kt * 128 + row;
-      const bool there = key < g.kv_len, sink = key < g.sinks;
+      const bool there = key < g.kv_len, sink = args.sink_tiles > 0 && key < g.sinks;
 #pragma unroll 1
       for (int m = 0; m < 2; ++m) {
         if (w.n > 0 && !wait(&sh.sum_full[m], (m == 0 ? kown : own) & 1u)) return;
         const uint32_t acc = tmem + lane_addr + (m == 0 ? C::DV : C::DK);
         const float f = m == 0 ? 1.f : args.scale;
-        if (p.kt * 128 < g.sinks) {
+        if (p.kt < args.sink_tiles) {
           float* part = sink ? kv_partial<D>(args, p.b, p.h, key, p.piece) + m * D : nullptr;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -1036,7 +1036,13 @@ GradPlan grad_plan(const AttnGeom& g, int dim) {
     const int64_t t_lo = std::max<int64_t>(0, -off);
     const int64_t next = std::max<int64_t>(t_hi < t_lo ? t_lo / g.tpt : t_hi / g.tpt + 1, 0);
     p.far_tiles = static_cast<int>((static_cast<int64_t>(g.window) + 128) / g.tpt + 1);
-    p.far_pieces = next >= g.tiles ? 0 : static_cast<int>(cdiv(g.tiles - next, p.far_tiles));
+    // Without a later tile there is nothing to join (3 x 250 tokens, W 100:
+    // 18.0 -> 16.3 us).  One or two later tiles are far pieces all the same: in
+    // the main piece they took longer than the join (3 x 333: 18.7 / 19.5).
+    if (next >= g.tiles)
+      p.sink_tiles = 0;
+    else
+      p.far_pieces = static_cast<int>(cdiv(g.tiles - next, p.far_tiles));
   }
   const uint64_t heads = static_cast<uint64_t>(g.batch) * g.heads_kv;
   p.stats_bytes = heads * g.tiles * 1024u;

@@ -90,6 +90,8 @@ WINDOW_CASES = [
     (1, 40, 40, 128, 1, 64, 16, 2),       # 128 heads: one token per tile
     (1, 37, 37, 100, 1, 64, None, 0),
     (3, 2050, 2050, 4, 1, 64, 256, 4),    # far pieces of the sinks' gradient
+    (2, 250, 250, 6, 2, 64, 100, 2),      # sinks whose window reaches the last token
+    (1, 300, 300, 4, 4, 128, 290, 140),   # the same, sinks in two key tiles
     (4, 1724, 1551, 8, 1, 64, 11, 4),     # whole tiles without a key between others
     (2, 6000, 500, 4, 1, 64, 100, 4),     # most tiles without a key
 ]
