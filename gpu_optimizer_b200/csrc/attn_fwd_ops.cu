@@ -450,8 +450,8 @@ __device__ __forceinline__ void fwd_barrier(int id) {
 
 // Joins the parts [c0, c1] of a unit with few rows (16 at most), in their
 // order and against a running maximum.  A thread has every nx-th vector of four
-// dims of one row; those of 16 parts are loaded before the first is used, as
-// the loop is bound by the latency of these loads (one token over 8K: 15.2 us,
+// dims of one row; those of P parts are loaded before the first is used, as
+// the loop is bound by the latency of these loads (one token over 8K: 15.1 us,
 // with 8 parts of two vectors 16.2; 16 parts of two spill).
 template <typename LoadMl, typename Load, typename Finish>
 __device__ __forceinline__ void fwd_join(int id, int rows, int vecs, int c0, int c1,
@@ -1064,8 +1064,10 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
           return __ldcg(reinterpret_cast<const float4*>(part_of(c)) + base + r +
                         x * args.part_rows);
         };
-        if (rows <= 16) {
-          fwd_join(row, rows, D / 4, c_first, c_last, load_ml, load, finish);
+        // with two tiles a unit has two or three parts, few rows or many
+        if (TILES == 1 && rows <= 16) {
+          if constexpr (TILES == 1)
+            fwd_join(row, rows, D / 4, c_first, c_last, load_ml, load, finish);
         } else if (row < rows) {
           // thread = row: its weights first, then 32 dims of two parts at a
           // time (16 loads in flight), which leave as 32-byte stores
@@ -1278,8 +1280,8 @@ int fwd_spans(const AttnGeom& g) {
 // over 2 x 128K 98 / 1097, over 64 x 0.8K..8K 191 / 232; chunks of up to 300
 // over 12 x 1.2K..6K, window 1024, 20.2 / 40.2; 4 chunks of 512 over 8K
 // 231 / 237.  Where lengths happen to fill the rounds, whole units would win
-// (single tokens over 128 x 2K 116 / 109, 16 chunks of 512 over 2K 231 / 206),
-// but the lengths are on the device: cutting loses 12 % at most, whole units
+// (single tokens over 128 x 2K 116 / 109, 16 chunks of 512 over 2K 236 / 206),
+// but the lengths are on the device: cutting lost 15 % at most, whole units
 // lose any factor.
 bool fwd_is_cut(const AttnGeom& g) {
   const int64_t pairs = static_cast<int64_t>(fwd_spans(g)) * g.batch;
