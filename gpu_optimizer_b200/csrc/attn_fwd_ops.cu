@@ -49,11 +49,11 @@
 //                                  exp2 -> P -> PV, twice, half overlapped
 //   4 x 4096 causal                495 us, 1110 TFLOP/s, as above
 //   64 single tokens, 0.8K..8K     191 us, 0.91 of the copy rate: HBM
-//   2 single tokens, 4 kv heads,   98 us, 0.83 of it: HBM, and SMs that end up
+//   2 single tokens, 4 kv heads,   97 us, 0.84 of it: HBM, and SMs that end up
 //     128K                         to a third before the last
 //   one token over 777             11 us: launch, a chain of dependent loads
 //                                  (length, page, K, V) and the join
-//   4 chunks of 512 over 8K        231 us, 1030 TFLOP/s; as the prefill
+//   4 chunks of 512 over 8K        234 us, 1030 TFLOP/s; as the prefill
 #include <algorithm>
 
 #include "attn_ops.cuh"
