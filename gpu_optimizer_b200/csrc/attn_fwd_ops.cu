@@ -9,7 +9,7 @@
 // and kv head (attn_ops.cuh: a tile packs all query heads of the kv head,
 // so K/V is read once for all of them).  One persistent CTA per SM:
 //   warp 0     TMA of Q and of the K ring
-//   warp 3     TMA of the V ring; clears V rows behind a sequence's last key
+//   warp 3     TMA of the V ring; clears V rows of keys that no row may weigh
 //   warp 1     MMA issuer; P overlays S in TMEM as 16-bit pairs
 //   warp 2     TMEM owner; walks the CTA's stretches and hands them out; sends
 //              staged tiles of O to memory
@@ -27,8 +27,9 @@
 // advances.)
 //
 // Only blocks with a visible key are loaded.  A page that ends inside a
-// block is loaded as boxes of its own rows; boxes without a key are asked
-// for outside the tensor, which TMA fills with zeros.
+// block is loaded as boxes of its own rows; boxes without a key, or whose keys
+// no token of the sequence sees, are asked for outside the tensor, which TMA
+// fills with zeros.
 //
 // Whole units (many of them) are dealt out in rounds, the longest rows first
 // and every other round backwards.  Few units (STREAM, paged only) are cut:
@@ -109,7 +110,7 @@ struct FwdShared {
   uint64_t q_full, q_empty;
   uint64_t k_full[kFwdMaxStages], k_empty[kFwdMaxStages];
   uint64_t v_full[kFwdMaxStages], v_empty[kFwdMaxStages];
-  uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared behind the last key
+  uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared (fwd_clears)
   uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], p_half[2], pv_done[kFwdSBufs];
   uint64_t o_full[2], o_free[2];
   // One staging tile for both tiles of O.  Use u has been stored when phase
@@ -507,6 +508,15 @@ struct FwdGeom {
   static constexpr uint32_t KV_BYTES = static_cast<uint32_t>(kOpsBN) * D * 2;
 };
 
+// Whether rows of a V block are cleared before the MMA reads it: slots behind
+// a sequence's last key (paged; dense copies end there) and keys that no token
+// sees hold anything.  P is 0 there, but 0 * NaN is not.
+template <bool PAGED>
+__device__ __forceinline__ bool fwd_clears(const AttnGeom& g, const AttnSeq& s, int key0) {
+  return (PAGED && key0 + kOpsBN > s.kv_len) ||
+         (key0 < s.unseen && attn_unseen_rows(g, s, key0).any());
+}
+
 // ---------------------------------------------------------------- producer
 // K ring and Q (is_k), or V ring.  The whole warp runs the loop: each lane
 // loads one box of a block.
@@ -526,6 +536,35 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
   RingPos2 pos;
   uint32_t taken = 0;
   FwdSeg s;
+  // The V block (its first key, -1: none) that is copied and not yet cleared.
+  // It is cleared when the next slot of the ring is not free, so that the
+  // blocks behind it are on their way meanwhile.
+  int dirty = -1;
+  RingPos2 dirty_at;
+  auto clear = [&]() {
+    if (dirty < 0) return true;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[dirty_at.slot]), dirty_at.parity,
+                                           abort_flag, args.err, kErrWaitProducer)))
+      return false;
+    const uint32_t slot = ring + dirty_at.slot * G::KV_BYTES;
+    constexpr int VECS = G::ATOMS * 8, ROWS = 32 / VECS;  // of a row; rows of a pass
+    auto rows = [&](int r0, int r1) {
+      for (int r = r0 + lane / VECS; r < r1; r += ROWS)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                         slot + (lane % VECS / 8) * kOpsBN * G::SW + r * G::SW + (lane % 8) * 16),
+                     "r"(0)
+                     : "memory");
+    };
+    const AttnUnseenRows u = attn_unseen_rows(g, s.seq, dirty);
+    rows(u.a0, u.a1);
+    rows(u.b0, u.b1);
+    if (PAGED) rows(s.seq.kv_len - dirty, kOpsBN);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[dirty_at.slot]));
+    dirty = -1;
+    return true;
+  };
   while (fwd_take<true>(sh, taken, s, args.err, kErrWaitProducer, ok)) {
     fwd_taken<true>(sh, taken);
     if (s.i0 == s.i1) continue;
@@ -553,12 +592,17 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
       if constexpr (PAGED) {
         const int key = key0 + lane * g.box_rows;
         page = g.num_pages;  // outside the tensor: zeros
-        if (lane < boxes && key < s.seq.kv_len)
+        if (lane < boxes && key < s.seq.kv_len && !attn_box_unseen(g, s.seq, key))
           page = __ldg(g.table + s.b * g.table_stride + key / g.page_size);
         row = key % g.page_size;
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[pos.slot]), pos.parity ^ 1u,
-                                             abort_flag, args.err, kErrWaitProducer));
+      const uint32_t free = smem_u32(&empty[pos.slot]);
+      if (dirty >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(free, pos.parity ^ 1u))) {
+        ok = clear();
+        if (!ok) break;
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(free, pos.parity ^ 1u, abort_flag, args.err,
+                                             kErrWaitProducer));
       if (!ok) break;
       const uint32_t bar = smem_u32(&full[pos.slot]);
       const uint32_t slot = ring + pos.slot * G::KV_BYTES;
@@ -571,25 +615,15 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
           tma_load_4d(dst + c * kOpsBN * G::SW, map, bar, c * 64, s.h, row, page);
       }
       ++issued;
-      if (PAGED && !is_k && key0 + kOpsBN > s.seq.kv_len) {
-        // Slots behind a sequence's last key hold anything; P is 0 there,
-        // but 0 * NaN is not: their V rows are cleared in shared memory
-        // before the MMA reads the block (always a unit's last one).
-        ok = __all_sync(0xffffffffu,
-                        mbar_wait(bar, pos.parity, abort_flag, args.err, kErrWaitProducer));
+      if (!is_k && fwd_clears<PAGED>(g, s.seq, key0)) {
+        ok = clear();
         if (!ok) break;
-        for (int r = s.seq.kv_len - key0; r < kOpsBN; ++r)
-          if (lane < G::ATOMS * 8)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             slot + (lane / 8) * kOpsBN * G::SW + r * G::SW + (lane % 8) * 16),
-                         "r"(0)
-                         : "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[pos.slot]));
+        dirty = key0;
+        dirty_at = pos;
       }
       pos.step(stages);
     }
+    if (ok) ok = clear();
     if (!ok) break;
   }
   if (!ok && lane == 0) {
@@ -642,7 +676,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
   uint32_t cleaned = 0;  // bit s: parity of slot s's next v_clean phase
   auto wait_v = [&](const FwdSeg& s, int i) {
     if (!wait(&sh.v_full[vpos.slot], vpos.parity)) return false;
-    if (PAGED && (s.blk.at(i) + 1) * BN > s.seq.kv_len) {
+    if (fwd_clears<PAGED>(args.geom, s.seq, s.blk.at(i) * BN)) {
       if (!wait(&sh.v_clean[vpos.slot], (cleaned >> vpos.slot) & 1u)) return false;
       cleaned ^= 1u << vpos.slot;
     }

@@ -40,7 +40,12 @@ struct AttnSeq {
   int q_len, kv_len;
   int row0;  // first row of the sequence in the packed q (paged), else 0
   int off;   // position of token 0
+  int unseen;  // keys [sinks, unseen) are in front of every token's window
 };
+
+__device__ __forceinline__ int attn_unseen(const AttnGeom& g, int off) {
+  return max(0, off - g.window + 1);
+}
 
 // Lengths of sequence b.  Paged lengths are device data that the host has
 // not seen: values that do not fit the buffers are cut to what does.
@@ -66,6 +71,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnGeom& g, int b, unsigned i
     s.kv_len = g.kv_len;
   }
   s.off = s.kv_len - s.q_len;
+  s.unseen = attn_unseen(g, s.off);
   return s;
 }
 
@@ -88,6 +94,26 @@ __device__ __forceinline__ AttnBlocks attn_blocks(const AttnGeom& g, const AttnS
   b.sink_blocks = min(b.first, (min(g.sinks, hi + 1) + kOpsBN - 1) / kOpsBN);
   b.n = b.sink_blocks + hi / kOpsBN - b.first + 1;
   return b;
+}
+
+// What a key holds that no token of its sequence sees must not reach a sum:
+// its weight is 0, but 0 * NaN is not.  Boxes (box_rows keys, the unit of a
+// copy) of such keys alone are not copied; the others are cleared in shared
+// memory.  Dense blocks are one box, and none without a visible key is loaded.
+__device__ __forceinline__ bool attn_box_unseen(const AttnGeom& g, const AttnSeq& s, int key) {
+  return key >= g.sinks && key + g.box_rows <= s.unseen;
+}
+// Rows of the block at key0 to clear, [a0, a1) behind the sinks and [b0, b1)
+// in front of the window (either may be empty, both may overlap).
+struct AttnUnseenRows {
+  int a0, a1, b0, b1;
+  __device__ __forceinline__ bool any() const { return a0 < a1 || b0 < b1; }
+};
+__device__ __forceinline__ AttnUnseenRows attn_unseen_rows(const AttnGeom& g, const AttnSeq& s,
+                                                           int key0) {
+  const int a = max(key0, g.sinks), b = min(key0 + kOpsBN, s.unseen), box = g.box_rows - 1;
+  return AttnUnseenRows{a - key0, min(b, (a + box) & ~box) - key0, max(a, b & ~box) - key0,
+                        b - key0};
 }
 
 // Bits [a, b) of word c of a 32-bit mask row (bit i of word c is index 32c + i).
