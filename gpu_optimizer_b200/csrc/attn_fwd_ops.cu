@@ -110,7 +110,7 @@ struct FwdShared {
   uint64_t q_full, q_empty;
   uint64_t k_full[kFwdMaxStages], k_empty[kFwdMaxStages];
   uint64_t v_full[kFwdMaxStages], v_empty[kFwdMaxStages];
-  uint64_t v_clean[kFwdMaxStages];  // the slot's block is cleared (fwd_clears)
+  uint64_t v_raw[kFwdMaxStages];  // copied, to be cleared before v_full (fwd_clears)
   uint64_t s_full[kFwdSBufs], p_full[kFwdSBufs], p_half[2], pv_done[kFwdSBufs];
   uint64_t o_full[2], o_free[2];
   // One staging tile for both tiles of O.  Use u has been stored when phase
@@ -510,17 +510,20 @@ struct FwdGeom {
 
 // Whether rows of a V block are cleared before the MMA reads it: slots behind
 // a sequence's last key (paged; dense copies end there) and keys that no token
-// sees hold anything.  P is 0 there, but 0 * NaN is not.
-template <bool PAGED>
+// sees hold anything.  P is 0 there, but 0 * NaN is not.  The copy of such a
+// block ends at v_raw, and v_full is announced once it is cleared: the MMA
+// thread, whose pace the others follow, has no part in it.  UNSEEN: the problem
+// has keys that no token sees (paged: it may).
+template <bool PAGED, bool UNSEEN>
 __device__ __forceinline__ bool fwd_clears(const AttnGeom& g, const AttnSeq& s, int key0) {
   return (PAGED && key0 + kOpsBN > s.kv_len) ||
-         (key0 < s.unseen && attn_unseen_rows(g, s, key0).any());
+         (UNSEEN && key0 < attn_unseen(g, s) && attn_unseen_rows(g, s, key0).any());
 }
 
 // ---------------------------------------------------------------- producer
 // K ring and Q (is_k), or V ring.  The whole warp runs the loop: each lane
 // loads one box of a block.
-template <int D, bool PAGED, int TILES>
+template <int D, bool PAGED, bool UNSEEN, int TILES>
 __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
                                              const CUtensorMap* tma_q, const CUtensorMap* map,
                                              uint32_t q_smem, uint32_t ring, bool is_k, int lane) {
@@ -531,6 +534,7 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
   volatile int* abort_flag = &sh.abort;
   const int boxes = PAGED ? kOpsBN / g.box_rows : 1;
   const int stages = is_k ? args.k_stages : args.v_stages;
+  constexpr bool CLEARS = PAGED || UNSEEN;
   bool ok = true;
   int issued = 0, q_loads = 0;
   RingPos2 pos;
@@ -539,14 +543,17 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
   // The V block (its first key, -1: none) that is copied and not yet cleared.
   // It is cleared when the next slot of the ring is not free, so that the
   // blocks behind it are on their way meanwhile.
-  int dirty = -1;
-  RingPos2 dirty_at;
+  int dirty = -1, dirty_slot = 0;
+  uint32_t raw = 0, held = 0;  // bit s: parity of slot s's next v_raw phase; not cleared yet
   auto clear = [&]() {
     if (dirty < 0) return true;
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[dirty_at.slot]), dirty_at.parity,
-                                           abort_flag, args.err, kErrWaitProducer)))
+    if (!__all_sync(0xffffffffu,
+                    mbar_wait(smem_u32(&sh.v_raw[dirty_slot]), (raw >> dirty_slot) & 1u,
+                              abort_flag, args.err, kErrWaitProducer)))
       return false;
-    const uint32_t slot = ring + dirty_at.slot * G::KV_BYTES;
+    raw ^= 1u << dirty_slot;
+    held &= ~(1u << dirty_slot);
+    const uint32_t slot = ring + dirty_slot * G::KV_BYTES;
     constexpr int VECS = G::ATOMS * 8, ROWS = 32 / VECS;  // of a row; rows of a pass
     auto rows = [&](int r0, int r1) {
       for (int r = r0 + lane / VECS; r < r1; r += ROWS)
@@ -561,7 +568,7 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
     if (PAGED) rows(s.seq.kv_len - dirty, kOpsBN);
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sh.v_clean[dirty_at.slot]));
+    if (lane == 0) mbar_arrive(smem_u32(&full[dirty_slot]));
     dirty = -1;
     return true;
   };
@@ -596,15 +603,16 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
           page = __ldg(g.table + s.b * g.table_stride + key / g.page_size);
         row = key % g.page_size;
       }
+      const bool clears = !is_k && fwd_clears<PAGED, UNSEEN>(g, s.seq, key0);
+      const uint32_t bar = smem_u32(clears ? &sh.v_raw[pos.slot] : &full[pos.slot]);
       const uint32_t free = smem_u32(&empty[pos.slot]);
-      if (dirty >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(free, pos.parity ^ 1u))) {
+      if (CLEARS && dirty >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(free, pos.parity ^ 1u))) {
         ok = clear();
         if (!ok) break;
       }
       ok = __all_sync(0xffffffffu, mbar_wait(free, pos.parity ^ 1u, abort_flag, args.err,
                                              kErrWaitProducer));
       if (!ok) break;
-      const uint32_t bar = smem_u32(&full[pos.slot]);
       const uint32_t slot = ring + pos.slot * G::KV_BYTES;
       if (lane == 0) mbar_arrive_expect_tx(bar, G::KV_BYTES);
       __syncwarp();
@@ -615,22 +623,28 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
           tma_load_4d(dst + c * kOpsBN * G::SW, map, bar, c * 64, s.h, row, page);
       }
       ++issued;
-      if (!is_k && fwd_clears<PAGED>(g, s.seq, key0)) {
-        ok = clear();
-        if (!ok) break;
+      if (CLEARS && clears) {
+        ok = clear();  // the one before
         dirty = key0;
-        dirty_at = pos;
+        dirty_slot = pos.slot;
+        held |= 1u << pos.slot;
+        if (!ok) break;
       }
       pos.step(stages);
     }
-    if (ok) ok = clear();
+    if (CLEARS && ok) ok = clear();
     if (!ok) break;
   }
   if (!ok && lane == 0) {
     // let the copies in flight land before the CTA can exit
     if (q_loads > 0) mbar_wait_drain(smem_u32(&sh.q_full), (q_loads - 1) & 1u, args.err);
-    for (int j = max(0, issued - stages); j < issued; ++j)
-      mbar_wait_drain(smem_u32(&full[j % stages]), (j / stages) & 1u, args.err);
+    for (int j = max(0, issued - stages); j < issued; ++j) {
+      const int at = j % stages;
+      if (CLEARS && !is_k && ((held >> at) & 1u))
+        mbar_wait_drain(smem_u32(&sh.v_raw[at]), (raw >> at) & 1u, args.err);
+      else
+        mbar_wait_drain(smem_u32(&full[at]), (j / stages) & 1u, args.err);
+    }
   }
 }
 
@@ -673,15 +687,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
   };
   bool ok = true;
   RingPos2 kpos, vpos;
-  uint32_t cleaned = 0;  // bit s: parity of slot s's next v_clean phase
-  auto wait_v = [&](const FwdSeg& s, int i) {
-    if (!wait(&sh.v_full[vpos.slot], vpos.parity)) return false;
-    if (fwd_clears<PAGED>(args.geom, s.seq, s.blk.at(i) * BN)) {
-      if (!wait(&sh.v_clean[vpos.slot], (cleaned >> vpos.slot) & 1u)) return false;
-      cleaned ^= 1u << vpos.slot;
-    }
-    return true;
-  };
+  auto wait_v = [&]() { return wait(&sh.v_full[vpos.slot], vpos.parity); };
   uint32_t segs = 0, taken = 0;
   FwdSeg s;
   if constexpr (TILES == 1) {
@@ -706,7 +712,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
         }
         const int j = i - LAG;
         if (j >= 0) {
-          ok = wait_v(s, s.i0 + j) && wait(&sh.p_full[ppos.slot], ppos.parity);
+          ok = wait_v() && wait(&sh.p_full[ppos.slot], ppos.parity);
           // the first PV overwrites O: the last epilogue has read it
           if (ok && j == 0 && segs > 0) ok = wait(&sh.o_free[0], (segs - 1) & 1u);
           if (!ok) break;
@@ -750,7 +756,7 @@ __device__ __forceinline__ void fwd_mma(const FwdArgs& args, FwdShared& sh, uint
         const bool more = i + 1 < s.i1;
 #pragma unroll
         for (int t = 0; t < 2; ++t) then[t] = more && sees(t, i + 1);
-        ok = wait_v(s, i);
+        ok = wait_v();
         if (!ok) break;
         bool k_ready = false;
 #pragma unroll
@@ -1161,7 +1167,7 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
   }
 }
 
-template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
+template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES, bool UNSEEN>
 __global__ void __launch_bounds__(128 + 128 * TILES, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q,
                     const __grid_constant__ CUtensorMap tma_k,
@@ -1189,7 +1195,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
       mbar_init(smem_u32(&sh.k_empty[s]), 1);
       mbar_init(smem_u32(&sh.v_full[s]), 1);
       mbar_init(smem_u32(&sh.v_empty[s]), 1);
-      mbar_init(smem_u32(&sh.v_clean[s]), 1);
+      mbar_init(smem_u32(&sh.v_raw[s]), 1);
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(smem_u32(&sh.s_full[b]), 1);
@@ -1233,7 +1239,7 @@ __global__ void __launch_bounds__(128 + 128 * TILES, 1)
   if (warp < 4) {
     if constexpr (TILES == 2) fwd_regs_dec<kFwdLowRegs>();
     if (warp == 0 || warp == 3)
-      fwd_producer<D, PAGED, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
+      fwd_producer<D, PAGED, UNSEEN, TILES>(args, sh, &tma_q, warp == 0 ? &tma_k : &tma_v, q_smem,
                                     warp == 0 ? k_smem : v_smem, warp == 0, lane);
     else if (warp == 1 && elect_one())
       fwd_mma<FMT, D, PAGED, TILES>(args, sh, tmem, q_smem, k_smem, v_smem);
@@ -1332,7 +1338,7 @@ uint64_t fwd_counter_bytes(const AttnGeom& g) {
   return (static_cast<uint64_t>(8 * kFwdMaxCtas) + g.heads_kv) * 2u * sizeof(unsigned int);
 }
 
-template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES>
+template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES, bool UNSEEN = PAGED>
 gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   const AttnGeom& g = p.geom;
   CUtensorMap mq, mk, mv, mo;
@@ -1369,7 +1375,7 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
     a.part_rows = fwd_part_rows(g);
     ctas = sms;
   }
-  auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES>;
+  auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES, UNSEEN>;
   const uint32_t dyn =
       (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN +
        (TILES == 2 ? 128u : 0u)) * D * 2u + 1024u;
@@ -1382,6 +1388,9 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
 template <typename T, int FMT, int D>
 gpo_status run_fwd_form(const AttnProblem& p, const LaunchCtx& c) {
   const bool two = fwd_tiles(p.geom) == 2;
+  if (!p.paged && attn_has_unseen(p.geom))
+    return two ? run_fwd<T, FMT, D, false, false, 2, true>(p, c)
+               : run_fwd<T, FMT, D, false, false, 1, true>(p, c);
   if (!p.paged)
     return two ? run_fwd<T, FMT, D, false, false, 2>(p, c)
                : run_fwd<T, FMT, D, false, false, 1>(p, c);

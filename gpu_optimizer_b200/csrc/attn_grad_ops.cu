@@ -327,7 +327,7 @@ __device__ __forceinline__ QItem q_item(const GradArgs& a, int item) {
   it.h = (item - a.kv_items) % g.heads_kv;
   it.b = r % g.batch;
   it.tile = g.tiles - 1 - r / g.batch;  // the longest rows first
-  it.seq = AttnSeq{g.q_len, g.kv_len, 0, g.kv_len - g.q_len, attn_unseen(g, g.kv_len - g.q_len)};
+  it.seq = AttnSeq{g.q_len, g.kv_len, 0, g.kv_len - g.q_len};
   it.t0 = it.tile * g.tpt;
   it.t1 = min(it.t0 + g.tpt, g.q_len);
   it.blk = attn_blocks(g, it.seq, it.t0, it.t1);

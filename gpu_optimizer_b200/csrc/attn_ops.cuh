@@ -40,12 +40,7 @@ struct AttnSeq {
   int q_len, kv_len;
   int row0;  // first row of the sequence in the packed q (paged), else 0
   int off;   // position of token 0
-  int unseen;  // keys [sinks, unseen) are in front of every token's window
 };
-
-__device__ __forceinline__ int attn_unseen(const AttnGeom& g, int off) {
-  return max(0, off - g.window + 1);
-}
 
 // Lengths of sequence b.  Paged lengths are device data that the host has
 // not seen: values that do not fit the buffers are cut to what does.
@@ -71,7 +66,6 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnGeom& g, int b, unsigned i
     s.kv_len = g.kv_len;
   }
   s.off = s.kv_len - s.q_len;
-  s.unseen = attn_unseen(g, s.off);
   return s;
 }
 
@@ -96,12 +90,16 @@ __device__ __forceinline__ AttnBlocks attn_blocks(const AttnGeom& g, const AttnS
   return b;
 }
 
+// Keys [sinks, attn_unseen) are in front of every token's window.
+__device__ __forceinline__ int attn_unseen(const AttnGeom& g, const AttnSeq& s) {
+  return max(0, s.off - g.window + 1);
+}
 // What a key holds that no token of its sequence sees must not reach a sum:
 // its weight is 0, but 0 * NaN is not.  Boxes (box_rows keys, the unit of a
 // copy) of such keys alone are not copied; the others are cleared in shared
 // memory.  Dense blocks are one box, and none without a visible key is loaded.
 __device__ __forceinline__ bool attn_box_unseen(const AttnGeom& g, const AttnSeq& s, int key) {
-  return key >= g.sinks && key + g.box_rows <= s.unseen;
+  return key >= g.sinks && key + g.box_rows <= attn_unseen(g, s);
 }
 // Rows of the block at key0 to clear, [a0, a1) behind the sinks and [b0, b1)
 // in front of the window (either may be empty, both may overlap).
@@ -111,7 +109,8 @@ struct AttnUnseenRows {
 };
 __device__ __forceinline__ AttnUnseenRows attn_unseen_rows(const AttnGeom& g, const AttnSeq& s,
                                                            int key0) {
-  const int a = max(key0, g.sinks), b = min(key0 + kOpsBN, s.unseen), box = g.box_rows - 1;
+  const int a = max(key0, g.sinks), b = min(key0 + kOpsBN, attn_unseen(g, s));
+  const int box = g.box_rows - 1;
   return AttnUnseenRows{a - key0, min(b, (a + box) & ~box) - key0, max(a, b & ~box) - key0,
                         b - key0};
 }
@@ -308,6 +307,17 @@ inline gpo_status launch_in_order(void (*kernel)(K...), unsigned grid, unsigned 
     return GPO_LAUNCH_ERROR;
   }
   return launch_status();
+}
+
+// Whether a dense problem has keys that no token sees (attn_unseen).  Its
+// kernels are instances of their own: the tests of the blocks' positions in
+// loops that never clear one took 153.4 in place of 150.5 us (prompt of 8192,
+// W 1024) and 28.9 in place of 28.4 (3 x 333 tokens, forward and gradient).
+// Clearing costs 91.9 -> 94.4 us forward and 246 -> 256 back for 4096 queries
+// behind 4096 more keys, W 1024, 4 sinks, 32 heads over 8 of D 128.
+inline bool attn_has_unseen(const AttnGeom& g) {
+  const int64_t off = static_cast<int64_t>(g.kv_len) - g.q_len;
+  return g.q_len > 0 && off - g.window + 1 > g.sinks;
 }
 
 // Whether every row of `t` starts on 32 bytes (see store_pairs8).
