@@ -145,6 +145,8 @@ struct GradWork {
 struct GradShared {
   uint64_t own_full[2], own_empty[2];
   uint64_t a_full[kGradA], a_empty[kGradA];
+  uint64_t a_raw[kGradA];  // K copied, to be cleared before a_full (grad_clears)
+  uint64_t a_cleared;      // the storing warps' parts of it
   uint64_t b_full[kGradB], b_empty[kGradB];
   uint64_t st_full[2], st_empty[2];  // row statistics (key tiles)
   uint64_t s_full[2], dp_full;       // key tiles use s_full[0] alone
@@ -178,6 +180,8 @@ __device__ __forceinline__ void grad_init(GradShared& sh) {
   init(sh.own_empty, 2, 1);
   init(sh.a_full, kGradA, 1);
   init(sh.a_empty, kGradA, 1);
+  init(sh.a_raw, kGradA, 1);
+  init(&sh.a_cleared, 1, kGradOutWarps);
   init(sh.b_full, kGradB, 1);
   init(sh.b_empty, kGradB, 1);
   init(sh.st_full, 2, 1);
@@ -194,6 +198,15 @@ __device__ __forceinline__ void grad_init(GradShared& sh) {
   init(&sh.drain, 1, 1);
   sh.abort = 0;
   fence_barrier_init();
+}
+
+// Whether rows of a K block of ring A are cleared before the MMAs read it:
+// keys that no token sees hold anything, and 0 * NaN is not 0 in dS K.  The copy
+// of such a block ends at a_raw; the storing warps clear it and announce
+// a_full, so that no other role has a part in it.  UNSEEN instances alone
+// (attn_has_unseen).
+__device__ __forceinline__ bool grad_clears(const AttnGeom& g, const QItem& q, int key0) {
+  return key0 < attn_unseen(g, q.seq) && attn_unseen_rows(g, q.seq, key0).any();
 }
 
 template <int N>
@@ -376,7 +389,7 @@ struct GradMaps {
 // ---------------------------------------------------------------- producers
 // Side 0: own tile K (key tiles) or Q, ring A of Q + statistics, or of K.
 // Side 1: own tile V or dO, ring B of dO or V.
-template <int D, int SIDE>
+template <int D, int SIDE, bool UNSEEN>
 __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& sh,
                                               const GradMaps& maps, uint32_t base) {
   using G = GradGeom<D>;
@@ -393,6 +406,7 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
     return mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitProducer);
   };
   // 128 keys from `row`, or the rows of a query tile
+  uint32_t raw = 0, raw_parity = 0;  // bit s: slot s's last copy ends at a_raw; its parity
   auto load_keys = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int h, int row, int b) {
     mbar_arrive_expect_tx(smem_u32(bar), G::TILE);
 #pragma unroll
@@ -446,13 +460,21 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
         ok = false;
         break;
       }
-      const uint32_t dst = ring + pos.slot * G::TILE;
-      if (keys)
+      const uint32_t dst = ring + pos.slot * G::TILE, bit = 1u << pos.slot;
+      if (UNSEEN) raw &= ~bit;
+      if (keys) {
         load_rows(dst, SIDE == 0 ? maps.q : maps.dout, &full[pos.slot], p.h,
                   (p.first + j) * g.tpt, p.b);
-      else
-        load_keys(dst, SIDE == 0 ? maps.k : maps.v, &full[pos.slot], qi.h, qi.blk.at(j) * 128,
-                  qi.b);
+      } else {
+        const int key0 = qi.blk.at(j) * 128;
+        uint64_t* bar = &full[pos.slot];
+        if (UNSEEN && SIDE == 0 && grad_clears(g, qi, key0)) {
+          bar = &sh.a_raw[pos.slot];
+          raw |= bit;
+          raw_parity ^= bit;
+        }
+        load_keys(dst, SIDE == 0 ? maps.k : maps.v, bar, qi.h, key0, qi.b);
+      }
       ++issued;
       pos.step();
       if (SIDE == 0 && keys && !load_stats(p.b, p.h, p.first + j)) {
@@ -465,8 +487,13 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
   if (!ok) {
     // let the copies in flight land before the CTA can exit
     if (own > 0) mbar_wait_drain(smem_u32(&sh.own_full[SIDE]), (own - 1) & 1u, err);
-    for (int j = max(0, issued - N); j < issued; ++j)
-      mbar_wait_drain(smem_u32(&full[j % N]), (j / N) & 1u, err);
+    for (int j = max(0, issued - N); j < issued; ++j) {
+      const int at = j % N;
+      if (UNSEEN && ((raw >> at) & 1u))  // raw_parity has turned once more than the phase it waits for
+        mbar_wait_drain(smem_u32(&sh.a_raw[at]), ((raw_parity >> at) & 1u) ^ 1u, err);
+      else
+        mbar_wait_drain(smem_u32(&full[at]), (j / N) & 1u, err);
+    }
     for (int j = max(0, stats - 2); j < stats; ++j)
       mbar_wait_drain(smem_u32(&sh.st_full[j & 1]), (j >> 1) & 1u, err);
   }
@@ -836,10 +863,11 @@ struct GradEw {
 };
 
 // ---------------------------------------------------------- sums to memory
-// Thread = TMEM lane: a key's dV and dK, or a query row's dQ.
-template <typename T, int FMT, int D>
-__device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, uint32_t tmem,
-                                         int quarter, int lane) {
+// Thread = TMEM lane: a key's dV and dK, or a query row's dQ.  Before, K blocks
+// of a query tile are cleared where no token sees their keys (grad_clears).
+template <typename T, int FMT, int D, bool UNSEEN>
+__device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, uint32_t base,
+                                         uint32_t tmem, int quarter, int lane) {
   using C = GradTmem<D>;
   const AttnGeom& g = args.geom;
   const int row = quarter * 32 + lane;
@@ -858,8 +886,42 @@ __device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, u
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(bar));
   };
+  // tiles of ring A so far; bit s: parity of slot s's a_raw; blocks cleared
+  uint32_t steps = 0, raw_parity = 0, cleared = 0;
+  auto clear = [&](const QItem& it, int j) {
+    const int key0 = it.blk.at(j) * 128, slot = (steps + j) % kGradA;
+    if (!grad_clears(g, it, key0)) return true;
+    if (!wait(&sh.a_raw[slot], (raw_parity >> slot) & 1u)) return false;
+    raw_parity ^= 1u << slot;
+    const AttnUnseenRows u = attn_unseen_rows(g, it.seq, key0);
+    const uint32_t tile = base + GradGeom<D>::RING_A + slot * GradGeom<D>::TILE;
+    auto rows = [&](int r0, int r1) {
+      for (int i = row; i < (r1 - r0) * (D / 8); i += kGradOutWarps * 32) {
+        const int r = r0 + i / (D / 8), x = i % (D / 8);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                         tile + x / 8 * 128 * 128 + r * 128 + x % 8 * 16),
+                     "r"(0)
+                     : "memory");
+      }
+    };
+    rows(u.a0, u.a1);
+    rows(u.b0, u.b1);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.a_cleared));
+    if (quarter == 0) {
+      if (!wait(&sh.a_cleared, cleared & 1u)) return false;
+      if (lane == 0) mbar_arrive(smem_u32(&sh.a_full[slot]));
+    }
+    ++cleared;
+    return true;
+  };
   GradWork w;
   while (grad_take<true>(sh, taken, w, args.err, kErrWaitEpilogue, ok)) {
+    if (UNSEEN && w.kind == 2)
+      for (int j = 0; j < w.n; ++j)
+        if (!clear(w.q, j)) return;
+    if (UNSEEN) steps += w.n;
     if (w.kind == 1) {
       const KvPiece& p = w.p;
       const int key = p.kt * 128 + row;
@@ -911,7 +973,7 @@ __device__ __forceinline__ void grad_out(const GradArgs& args, GradShared& sh, u
   }
 }
 
-template <typename T, int FMT, int D>
+template <typename T, int FMT, int D, bool UNSEEN>
 __global__ void __launch_bounds__(kGradThreads, 1)
     attn_grad_kernel(const __grid_constant__ CUtensorMap tma_q,
                      const __grid_constant__ CUtensorMap tma_do,
@@ -966,13 +1028,13 @@ __global__ void __launch_bounds__(kGradThreads, 1)
   if (warp < 4) {
     grad_regs_dec<kGradLowRegs>();
     if (warp == 0) {
-      if (elect_one()) grad_producer<D, 0>(args, sh, maps, base);
+      if (elect_one()) grad_producer<D, 0, UNSEEN>(args, sh, maps, base);
     } else if (warp == 1) {
       if (elect_one()) grad_mma<FMT, D>(args, sh, base, tmem);
     } else if (warp == 2) {
       if (elect_one()) grad_schedule(args, sh);
     } else {
-      if (elect_one()) grad_producer<D, 1>(args, sh, maps, base);
+      if (elect_one()) grad_producer<D, 1, UNSEEN>(args, sh, maps, base);
     }
   } else if (warp < 12) {
     grad_regs_inc<kGradEwRegs>();
@@ -990,7 +1052,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     }
   } else {
     grad_regs_dec<kGradOutRegs>();
-    grad_out<T, FMT, D>(args, sh, tmem, warp & 3, lane);
+    grad_out<T, FMT, D, UNSEEN>(args, sh, base, tmem, warp & 3, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -1103,7 +1165,8 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
                                  static_cast<unsigned>(std::max<int64_t>(1, q_items)), 256, 0,
                                  c.stream, a);
   if (s != GPO_OK) return s;
-  auto kern = attn_grad_kernel<T, FMT, D>;
+  auto kern = attn_has_unseen(g) ? attn_grad_kernel<T, FMT, D, true>
+                                 : attn_grad_kernel<T, FMT, D, false>;
   constexpr uint32_t dyn = GradGeom<D>::BYTES;
   s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
