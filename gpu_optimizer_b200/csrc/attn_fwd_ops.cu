@@ -598,9 +598,15 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
       int page = s.b, row = key0;
       if constexpr (PAGED) {
         const int key = key0 + lane * g.box_rows;
-        page = g.num_pages;  // outside the tensor: zeros
-        if (lane < boxes && key < s.seq.kv_len && !attn_box_unseen(g, s.seq, key))
+        // a page outside the tensor arrives as zeros (that of a cache without
+        // pages has one all the same, as a tensor map cannot be empty)
+        const int outside = max(g.num_pages, 1);
+        page = outside;
+        if (lane < boxes && key < s.seq.kv_len && !attn_box_unseen(g, s.seq, key)) {
           page = __ldg(g.table + s.b * g.table_stride + key / g.page_size);
+          if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(g.num_pages))
+            page = outside;
+        }
         row = key % g.page_size;
       }
       const bool clears = !is_k && fwd_clears<PAGED, UNSEEN>(g, s.seq, key0);
