@@ -106,11 +106,13 @@ class PagedAttention:
     Per call, ``page_table`` (int32, seqs x width) names the page of every
     ``page_size`` slots of a sequence, ``q_start`` (int32, seqs + 1) the first
     row of each sequence in the packed rows, and ``kv_len`` (int32, seqs) its
-    keys, new tokens included.  Both stay on the device and are not read by
+    keys, new tokens included.  All stay on the device and are not read by
     the host; a sequence whose lengths do not fit the buffers is skipped and
     reported by ``runner.check_device_status``.  Page table entries behind a
     sequence's last key, and those of pages no token sees any more, are not
-    read as pages.
+    read as pages.  An entry outside the cache is not followed: ``append`` does
+    not write its rows, ``attend`` takes its keys and values as zeros and
+    reports it.
 
     The plan owns the kernels' workspace: calls of one plan have to follow
     one another on a stream; concurrent streams need a plan each.

@@ -604,8 +604,10 @@ __device__ __forceinline__ void fwd_producer(const FwdArgs& args, FwdShared& sh,
         page = outside;
         if (lane < boxes && key < s.seq.kv_len && !attn_box_unseen(g, s.seq, key)) {
           page = __ldg(g.table + s.b * g.table_stride + key / g.page_size);
-          if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(g.num_pages))
+          if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(g.num_pages)) {
             page = outside;
+            atomicOr(args.err, kErrBadLaunch);
+          }
         }
         row = key % g.page_size;
       }

@@ -19,12 +19,12 @@ struct AppendArgs {
   int64_t kn_token, kn_head, vn_token, vn_head;
   int64_t kp_page, kp_slot, kp_head, vp_page, vp_slot, vp_head;
   int vecs;  // vectors of a row
+  unsigned int* err;
 };
 
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+// One vector of a token's K and V.
+__device__ __forceinline__ void append_vector(const AppendArgs& a) {
   const AttnGeom& g = a.geom;
-  let_next_start();
-  wait_for_previous();
   const int per_token = g.heads_kv * a.vecs;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t t64 = i / per_token;
@@ -42,17 +42,31 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
       hi = m;
   }
   const int first = __ldg(g.q_start + lo), end = __ldg(g.q_start + lo + 1);
-  if (t < first || t >= end) return;
-  const int64_t slot = static_cast<int64_t>(__ldg(g.kv_lens + lo)) - (end - t);
-  const int64_t at = slot / g.page_size;
-  if (slot < 0 || at >= g.table_width) return;
+  const int keys = __ldg(g.kv_lens + lo);
+  // a sequence that does not fit (attn_seq) is not written, not even in part
+  if (t < first || t >= end || first < 0 || end > g.tokens ||
+      keys > g.table_width * g.page_size)
+    return;
+  const int slot = keys - (end - t);
+  if (slot < 0) return;  // a token in front of the first key has none
+  const int at = slot / g.page_size;
   const int page = __ldg(g.table + lo * g.table_stride + at);
   if (page < 0 || page >= g.num_pages) return;
-  const int64_t s = slot - at * g.page_size;
+  const int row = slot - at * g.page_size;
   const uint4 kv = __ldcs(a.k_new + t * a.kn_token + h * a.kn_head + x);
   const uint4 vv = __ldcs(a.v_new + t * a.vn_token + h * a.vn_head + x);
-  a.k_pages[page * a.kp_page + s * a.kp_slot + h * a.kp_head + x] = kv;
-  a.v_pages[page * a.vp_page + s * a.vp_slot + h * a.vp_head + x] = vv;
+  a.k_pages[page * a.kp_page + row * a.kp_slot + h * a.kp_head + x] = kv;
+  a.v_pages[page * a.vp_page + row * a.vp_slot + h * a.vp_head + x] = vv;
+}
+
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+  const AttnGeom& g = a.geom;
+  let_next_start();
+  wait_for_previous();
+  append_vector(a);
+  // sequences that do not fit are reported, those that no token leads to included
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < g.batch; b += 256) attn_seq<true>(g, b, a.err);
 }
 
 gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c) {
@@ -73,6 +87,8 @@ gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c) {
   a.vp_slot = p.v.s_token / 8;
   a.vp_head = p.v.s_head / 8;
   a.vecs = p.dim / 8;
+  a.err = c.err;
+  a.geom.q_len = a.geom.tokens;  // max_q bounds the attention's tiles, not a copy
   const uint64_t n = static_cast<uint64_t>(p.geom.tokens) * p.geom.heads_kv * a.vecs;
   const uint64_t blocks = cdiv(n, 256);
   if (blocks > 0x7fffffffull) return GPO_BAD_ARGS;

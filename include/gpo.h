@@ -291,14 +291,18 @@ GPO_API gpo_status gpo_window_workspace(const gpo_window_args* args, uint64_t* b
  * over its cache pages, which hold the new tokens' K/V already.  Lengths
  * and pages stay on the device: a sequence whose lengths do not fit the
  * buffers is skipped (its rows of out are not written) and reported by
- * gpo_device_status (bit 5); a page outside [0, num_pages) reads as zeros. */
+ * gpo_device_status (bit 5).  A page outside [0, num_pages) reads as zeros,
+ * and where a key of it is seen, that is reported in the same way. */
 GPO_API gpo_status gpo_paged_attention(const gpo_paged_args* args, void* stream, char* log,
                                        size_t log_cap);
 GPO_API gpo_status gpo_paged_workspace(const gpo_paged_args* args, uint64_t* bytes, char* log,
                                        size_t log_cap);
 /* Write the new tokens' rows k_new, v_new to the last slots of their
- * sequences: token i to slot kv_len - q_len + i.  Rows whose slot or page is
- * outside the buffers are not written. */
+ * sequences: token i to slot kv_len - q_len + i.  A sequence whose lengths do
+ * not fit the buffers (max_q does not count here) is skipped and reported by
+ * gpo_device_status (bit 5).  Rows without a slot (kv_len < q_len: the first
+ * ones) or whose page is outside [0, num_pages) are not written; the
+ * attention that reads such a page reports it. */
 GPO_API gpo_status gpo_cache_append(const gpo_paged_args* args, void* stream, char* log,
                                     size_t log_cap);
 
