@@ -35,8 +35,10 @@ bool check_common(int dtype, int dim, int hq, int hk, int64_t window, int64_t si
   if (hq / hk > 128)
     return r.no(GPO_BAD_CONFIG, "at most 128 query heads per kv head");
   if (window < 0 || sinks < 0) return r.no(GPO_BAD_ARGS, "window and sinks must not be negative");
-  if (!(scale >= 0.f) || !std::isfinite(scale))
-    return r.no(GPO_BAD_ARGS, "scale must be positive and finite");
+  // beyond, scale * log2(e) leaves the normal numbers and may meet a masked
+  // score as 0 * -inf
+  if (scale != 0.f && !(scale >= 0x1p-126f && scale <= 0x1p126f))
+    return r.no(GPO_BAD_ARGS, "scale must be positive and finite, in [2^-126, 2^126]");
   return true;
 }
 

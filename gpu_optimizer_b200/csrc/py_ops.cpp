@@ -7,7 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
-#include <cmath>
+#include <cstdio>
 #include <string>
 
 #include "gpo.h"
@@ -98,7 +98,12 @@ void set_mask(c10::optional<int64_t> window, int64_t sinks, c10::optional<double
   if (window && *window < 1)
     refuse("window must be at least 1 (or None), got " + std::to_string(*window));
   if (sinks < 0) refuse("sinks must not be negative, got " + std::to_string(sinks));
-  if (scale && !(*scale > 0)) refuse("scale must be positive, got " + std::to_string(*scale));
+  // as a float: what rounds to 0 would ask for the default
+  if (scale && !(static_cast<float>(*scale) > 0.f)) {
+    char text[64];
+    snprintf(text, sizeof(text), "scale must be positive (2^-126 at least), got %g", *scale);
+    refuse(text);
+  }
   w = window ? *window : 0;
   s = sinks;
   f = scale ? static_cast<float>(*scale) : 0.f;

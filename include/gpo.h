@@ -234,7 +234,8 @@ typedef struct gpo_window_args {
   int64_t batch, q_len, kv_len;
   int64_t window;      /* keys a query sees, its own included; 0: no window */
   int64_t sinks;       /* first keys that stay visible                      */
-  float scale;         /* of the scores; 0: 1 / sqrt(head_dim)              */
+  float scale;         /* of the scores, in [2^-126, 2^126];
+                          0: 1 / sqrt(head_dim)                             */
   int32_t reserved;    /* 0 */
   gpo_heads q, k, v;   /* inputs                                            */
   gpo_heads out;       /* forward: written; backward: read                  */
