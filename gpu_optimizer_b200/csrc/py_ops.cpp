@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <cstdint>
 #include <cstdio>
 #include <string>
 
@@ -58,6 +59,12 @@ void check_shape(const char* name, const Tensor& t, at::IntArrayRef want) {
   if (t.sizes() != want)
     refuse(std::string(name) + " has shape " + shape_of(t.sizes()) + ", expected " +
            shape_of(want));
+}
+
+// A size as the library's records hold it.
+int32_t size32(const char* name, int64_t n) {
+  if (n < 0 || n > INT32_MAX) refuse(std::string(name) + " is out of range: " + std::to_string(n));
+  return static_cast<int32_t>(n);
 }
 
 int dtype_id(at::ScalarType t) { return t == at::kBFloat16 ? GPO_BFLOAT16 : GPO_FLOAT16; }
@@ -144,9 +151,9 @@ gpo_window_args window_args(const Tensor& q, const Tensor& k, const Tensor& v,
            shape_of(v.sizes()) + " do not belong together");
   gpo_window_args a{};
   a.dtype = dtype_id(type);
-  a.head_dim = static_cast<int32_t>(q.size(3));
-  a.heads_q = static_cast<int32_t>(q.size(2));
-  a.heads_kv = static_cast<int32_t>(k.size(2));
+  a.head_dim = size32("head_dim", q.size(3));
+  a.heads_q = size32("heads_q", q.size(2));
+  a.heads_kv = size32("heads_kv", k.size(2));
   a.batch = q.size(0);
   a.q_len = q.size(1);
   a.kv_len = k.size(1);
@@ -238,9 +245,9 @@ struct Plan {
       refuse(std::string("dtype must be float16 or bfloat16, got ") + type_name(type));
     if (max_seqs < 1 || max_q < 1) refuse("max_seqs and max_q must be at least 1");
     args.dtype = dtype_id(type);
-    args.head_dim = static_cast<int32_t>(head_dim);
-    args.heads_q = static_cast<int32_t>(heads_q);
-    args.heads_kv = static_cast<int32_t>(heads_kv);
+    args.head_dim = size32("head_dim", head_dim);
+    args.heads_q = size32("heads_q", heads_q);
+    args.heads_kv = size32("heads_kv", heads_kv);
     args.page_size = page_size;
     args.max_q = max_q;
     args.num_seqs = max_seqs;

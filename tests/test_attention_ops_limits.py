@@ -33,3 +33,10 @@ def test_scales_below_the_normal_numbers_are_refused(scale):
     tiny = 2.0 ** -126
     assert call("gpo_window_workspace", window(scale=tiny), ctypes.c_uint64(0))[0] == _lib.OK
     assert math.isclose(tiny, 1.1754944e-38, rel_tol=1e-6)
+
+
+@pytest.mark.parametrize("bad", [{"heads_q": 2 ** 32 + 4}, {"heads_kv": 2 ** 32 + 2},
+                                 {"head_dim": 2 ** 32 + 64}, {"heads_q": -2 ** 32 + 4}])
+def test_sizes_that_32_bits_do_not_hold_are_refused(bad):
+    with pytest.raises(KernelBuildError, match=next(iter(bad))):
+        ops.PagedAttention(**{**PLAN, **bad})
