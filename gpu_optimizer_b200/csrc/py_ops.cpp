@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <string>
@@ -230,6 +231,8 @@ std::tuple<Tensor, Tensor, Tensor> window_backward(
 }
 
 // ------------------------------------------------------------------- paged
+constexpr int64_t kMostTokens = 1ll << 30;  // of a call (gpo.h)
+
 struct Plan {
   gpo_paged_args args{};
   at::ScalarType type;
@@ -251,7 +254,8 @@ struct Plan {
     args.page_size = page_size;
     args.max_q = max_q;
     args.num_seqs = max_seqs;
-    args.tokens = max_seqs * max_q;
+    // of all sequences at their longest, or what the library takes in one call
+    args.tokens = std::min<int64_t>(kMostTokens / max_seqs, max_q) * max_seqs;
     set_mask(window, sinks, scale, args.window, args.sinks, args.scale);
     char log[256];
     const gpo_status s = gpo_paged_workspace(&args, &args.workspace_bytes, log, sizeof(log));

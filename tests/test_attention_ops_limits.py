@@ -40,3 +40,17 @@ def test_scales_below_the_normal_numbers_are_refused(scale):
 def test_sizes_that_32_bits_do_not_hold_are_refused(bad):
     with pytest.raises(KernelBuildError, match=next(iter(bad))):
         ops.PagedAttention(**{**PLAN, **bad})
+
+
+def test_plans_may_allow_more_tokens_than_a_call_has():
+    """4096 sequences or chunks of 2^20 tokens, if not both in one call: the
+    plan is only refused for what a call could not hold alone."""
+    try:
+        ops.PagedAttention(**{**PLAN, "max_seqs": 4096, "max_q": 1 << 20})
+    except KernelBuildError as e:
+        pytest.fail(f"refused: {e}")
+    except (RuntimeError, AssertionError):
+        assert not torch.cuda.is_available()  # no device to allocate the workspace on
+    for bad in ({"max_seqs": 65536}, {"max_q": (1 << 30) + 1}, {"max_q": 1 << 62, "max_seqs": 4}):
+        with pytest.raises(KernelBuildError, match="num_seqs"):
+            ops.PagedAttention(**{**PLAN, **bad})
