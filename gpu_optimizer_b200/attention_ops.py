@@ -26,7 +26,8 @@ views); others are copied first.
 P and dS enter the tensor cores in the inputs' type (every sum is fp32).  With
 float16, dS below 2^-24 vanishes: scale the loss, as for any float16 training.
 
-Everything runs on torch's current stream and never synchronises.  A refused
+Everything runs on torch's current stream and, but for making a plan, never
+synchronises.  A refused
 argument raises ``KernelBuildError`` with the library's reason, before
 anything is launched; a launch that fails raises ``RuntimeError``.
 """
@@ -115,7 +116,9 @@ class PagedAttention:
     reports it.
 
     The plan owns the kernels' workspace: calls of one plan have to follow
-    one another on a stream; concurrent streams need a plan each.
+    one another, on a stream or ordered by events; concurrent streams need a
+    plan each.  Any stream may make the first call.  Making a plan waits for
+    its workspace (not for queued work), calls never wait.
     """
 
     def __init__(self, *, heads_q: int, heads_kv: int, head_dim: int, page_size: int,

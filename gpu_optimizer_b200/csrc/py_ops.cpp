@@ -3,6 +3,8 @@
 // (include/gpo.h).  It exists for the calls' latency: a single token's append
 // is a 4 us kernel behind a 5 us launch, and the same checks and records took
 // 13 us in Python.
+#include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -239,6 +241,7 @@ struct Plan {
   c10::Device device{c10::kCPU};
   int64_t max_seqs;
   Tensor work;
+  mutable c10::optional<c10::cuda::CUDAStream> held_by;  // the last call's stream
 
   Plan(int64_t heads_q, int64_t heads_kv, int64_t head_dim, int64_t page_size, int64_t max_seqs_,
        int64_t max_q, at::ScalarType type_, c10::optional<int64_t> window, int64_t sinks,
@@ -260,9 +263,34 @@ struct Plan {
     char log[256];
     const gpo_status s = gpo_paged_workspace(&args, &args.workspace_bytes, log, sizeof(log));
     if (s != GPO_OK) raise_status("gpo_paged_workspace", s, log);
-    work = at::zeros({static_cast<int64_t>(args.workspace_bytes)},
-                     at::TensorOptions().dtype(at::kByte).device(device));
+    make_workspace();
     args.workspace = work.data_ptr();
+  }
+
+  // The workspace is zero before the plan is handed out, whichever stream
+  // calls it first.  It is made on a stream of its own, which alone is waited
+  // for; in a capture the zeroing becomes a part of the graph.
+  void make_workspace() {
+    const auto bytes = static_cast<int64_t>(args.workspace_bytes);
+    const auto options = at::TensorOptions().dtype(at::kByte).device(device);
+    const c10::cuda::CUDAGuard on(device);
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+      work = at::zeros({bytes}, options);
+      return;
+    }
+    const auto own = c10::cuda::getStreamFromPool(false, device.index());
+    const c10::cuda::CUDAStreamGuard guard(own);
+    work = at::zeros({bytes}, options);
+    own.synchronize();
+  }
+
+  // Keeps the workspace from being handed on, if the plan is dropped, before
+  // the calls on this stream are done.
+  void hold_workspace() const {
+    const auto stream = c10::cuda::getCurrentCUDAStream(device.index());
+    if (held_by == stream) return;
+    c10::cuda::CUDACachingAllocator::recordStream(work.storage().data_ptr(), stream);
+    held_by = stream;
   }
 
   gpo_paged_args fill(int64_t rows, const Tensor& k_pages, const Tensor& v_pages,
@@ -333,6 +361,7 @@ struct Plan {
     a.q = heads3(q);
     a.out = heads3(out);
     a.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    hold_workspace();
     launch("gpo_paged_attention", gpo_paged_attention, a, device);
     return out;
   }
