@@ -59,12 +59,31 @@ def _native():
     return _ops
 
 
+class _NoGradient(torch.autograd.Function):
+    """Results (in a list, which torch does not look into) of a call that has
+    no gradient, for inputs that need one."""
+
+    @staticmethod
+    def forward(ctx, call, results, *inputs):
+        ctx.call = call
+        return tuple(r.detach() for r in results)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.call} has no gradient; window_attention is the differentiable "
+                           "form (call under torch.no_grad() where none is wanted)")
+
+
 def window_attention_forward(q, k, v, *, window: int | None = None, sinks: int = 0,
                              scale: float | None = None, out=None, lse=None):
     """(out, lse): attention of q over k, v, and each row's log-sum-exp of
     scaled scores, fp32 (batch, q_len, heads_q).  ``out`` and ``lse`` may name
-    the tensors to write."""
-    return (_ops or _native()).window_forward(q, k, v, window, sinks, scale, out, lse)
+    the tensors to write.  Not differentiable (``window_attention`` is): a
+    backward pass that reaches the results raises."""
+    results = (_ops or _native()).window_forward(q, k, v, window, sinks, scale, out, lse)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _NoGradient.apply("window_attention_forward", [*results], q, k, v)
+    return results
 
 
 def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = None,
@@ -72,10 +91,15 @@ def window_attention_backward(dout, q, k, v, out, lse, *, window: int | None = N
     """(dq, dk, dv) from the output's gradient and what the forward returned.
     ``grads`` may name the three tensors to write.
 
-    Sums run in a fixed order: the same inputs give the same bits.
+    Sums run in a fixed order: the same inputs give the same bits.  Not
+    differentiable once more.
     """
-    return (_ops or _native()).window_backward(dout, q, k, v, out, lse, window, sinks, scale,
-                                               grads)
+    results = (_ops or _native()).window_backward(dout, q, k, v, out, lse, window, sinks, scale,
+                                                  grads)
+    if torch.is_grad_enabled() and (dout.requires_grad or q.requires_grad or k.requires_grad
+                                    or v.requires_grad):
+        return _NoGradient.apply("window_attention_backward", [*results], dout, q, k, v)
+    return results
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -133,7 +157,8 @@ class PagedAttention:
 
     def append(self, k, v, k_pages, v_pages, page_table, q_start, kv_len) -> None:
         """Write the new tokens' rows k, v (tokens, heads_kv, head_dim) to the
-        last slots of their sequences: token i to kv_len - q_len + i."""
+        last slots of their sequences: token i to kv_len - q_len + i.  The
+        cache holds values: nothing is passed back through it."""
         self._plan.append(k, v, k_pages, v_pages, page_table, q_start, kv_len)
 
     def attend(self, q, k_pages, v_pages, page_table, q_start, kv_len, out=None,
@@ -141,8 +166,13 @@ class PagedAttention:
         """Attention of the new tokens q (tokens, heads_q, head_dim) over
         their sequences' pages; the tokens' own K/V are in the cache already.
         ``out`` may name the tensor to write, ``lse`` (fp32, tokens x heads_q)
-        one for the log-sum-exp."""
-        return self._plan.attend(q, k_pages, v_pages, page_table, q_start, kv_len, out, lse)
+        one for the log-sum-exp.  Not differentiable: a backward pass that
+        reaches the result raises."""
+        result = self._plan.attend(q, k_pages, v_pages, page_table, q_start, kv_len, out, lse)
+        if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad
+                                        or v_pages.requires_grad):
+            return _NoGradient.apply("PagedAttention.attend", [result], q, k_pages, v_pages)[0]
+        return result
 
 
 # ------------------------------------------------------- runner.build_callable
