@@ -8,7 +8,8 @@ into ``_build/`` at the repository root, the kernel sources are embedded for
 the static CUDA runtime into ``gpu_optimizer_b200/libgpo.so``.  A unit is
 rebuilt only when it, or a header it includes, is newer than its object.
 The operators' Python binding (``csrc/py_ops.cpp``, host C++ on torch's
-headers) becomes ``gpu_optimizer_b200/_ops.so`` next to it.
+headers) becomes ``gpu_optimizer_b200/_ops.so`` next to it, where torch is
+installed.
 """
 
 from __future__ import annotations
@@ -117,14 +118,21 @@ def build(jobs: int | None = None, verbose: bool = False, force: bool = False) -
     return LIB
 
 
-def build_binding(verbose: bool = False, force: bool = False) -> Path:
-    """Compile the operators' Python binding against the installed torch."""
+def build_binding(verbose: bool = False, force: bool = False) -> Path | None:
+    """Compile the operators' Python binding against the installed torch.
+
+    It is compiled again when its sources, torch, Python or the command
+    change (the last three are kept in ``_ops.so.key``).  Without torch there
+    is nothing to bind to and it is left out.
+    """
     src = CSRC / "py_ops.cpp"
-    if not force and not _stale(BINDING, src, [ROOT / "include" / "gpo.h"]):
-        return BINDING
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError as e:
+        print(f"the operators' binding is not built: {e}", file=sys.stderr)
+        return None
 
     base = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
@@ -137,12 +145,18 @@ def build_binding(verbose: bool = False, force: bool = False) -> Path:
            *(f"-isystem{p}" for p in includes), f"-I{ROOT / 'include'}", str(src), "-o", str(tmp),
            f"-L{base / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
            f"-L{PKG}", "-l:libgpo.so", "-Wl,-rpath,$ORIGIN"]
+    key_file = BINDING.with_suffix(".so.key")
+    key = "\n".join([torch.__version__, sys.version, *cmd])
+    if (not force and not _stale(BINDING, src, [ROOT / "include" / "gpo.h"])
+            and key_file.exists() and key_file.read_text() == key):
+        return BINDING
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose and (r.stdout or r.stderr):
         print(r.stdout + r.stderr, file=sys.stderr)
     if r.returncode != 0:
         raise RuntimeError(f"binding build failed:\n{r.stdout}{r.stderr}")
     os.replace(tmp, BINDING)
+    key_file.write_text(key)
     return BINDING
 
 
