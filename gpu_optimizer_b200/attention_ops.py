@@ -50,8 +50,11 @@ def _native():
     global _ops
     if _ops is None:
         try:
-            _lib.load()
+            abi = _lib.load().gpo_abi_version()
             ops = importlib.import_module(__package__ + "._ops")
+            if ops.ABI_VERSION != abi:
+                raise _lib.LibraryMissing(f"_ops.so is built for ABI {ops.ABI_VERSION}, "
+                                          f"libgpo.so has {abi}")
         except (_lib.LibraryMissing, ImportError) as e:
             raise KernelBuildError(str(e), log=str(e)) from e
         ops.set_refused(KernelBuildError)

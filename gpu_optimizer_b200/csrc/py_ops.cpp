@@ -371,7 +371,7 @@ struct Plan {
 
 PYBIND11_MODULE(_ops, m) {
   m.def("set_refused", [](py::object cls) { g_refused = std::move(cls); });
-  m.def("abi_version", &gpo_abi_version);
+  m.attr("ABI_VERSION") = GPO_ABI_VERSION;  // whose records this binding fills
   m.def("window_forward", &window_forward);
   m.def("window_backward", &window_backward);
   py::class_<Plan>(m, "Plan")

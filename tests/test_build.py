@@ -61,3 +61,20 @@ def test_library_is_built_without_torch(built, monkeypatch, capsys):
     assert b.build() == b.LIB
     assert "torch" in capsys.readouterr().err
     assert len(built) == 1 and not b.BINDING.exists()
+
+
+def test_binding_of_another_abi_is_refused(monkeypatch):
+    from gpu_optimizer_b200 import _lib, attention_ops
+    from gpu_optimizer_b200.runner import KernelBuildError
+
+    class Old:
+        ABI_VERSION = _lib.ABI_VERSION + 1
+
+        @staticmethod
+        def set_refused(cls):
+            pass
+
+    monkeypatch.setattr(attention_ops, "_ops", None)
+    monkeypatch.setattr(attention_ops.importlib, "import_module", lambda name: Old)
+    with pytest.raises(KernelBuildError, match="built for ABI"):
+        attention_ops._native()
