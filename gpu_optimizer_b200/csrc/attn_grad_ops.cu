@@ -7,14 +7,15 @@
 //   dQ = scale dS K                  dK = scale dS^T Q
 // with dK and dV summed over the query heads of a kv head.
 //
-// Two kernels: the rows' statistics (memory bound), and one persistent
-// kernel that first works through the key tiles (dK, dV) and then through
-// the query tiles (dQ).  The scores are computed in both (7 products in
-// place of 5), because each sum then has one owner and a fixed order: no
-// atomics on values, equal inputs give equal bits, and no fp32 copy of dQ
-// goes through memory.  P and dS are rounded to the inputs' type as MMA
-// operands; every sum is fp32 in TMEM.  (A third, small kernel joins the
-// sink keys' partial sums, see kv_piece.)
+// Three kernels: the rows' statistics (memory bound), one persistent kernel
+// that first works through the key tiles (dK, dV) and then through the query
+// tiles (dQ), and, where sink keys are seen from behind their window, a small
+// one that joins their partial sums (see kv_piece).  The scores are computed
+// for the key tiles and again for the query tiles (7 products in place of 5),
+// because each sum then has one owner and a fixed order: no atomics on values,
+// equal inputs give equal bits, and no fp32 copy of dQ goes through memory.
+// P and dS are rounded to the inputs' type as MMA operands; every sum is fp32
+// in TMEM.
 //
 // Roles of the persistent kernel, one CTA per SM:
 //   warp 0     TMA of the item's first own tile (K or Q), of ring A (Q or K)
@@ -58,8 +59,7 @@ struct GradArgs {
   int64_t o_batch, o_token, o_head, do_batch, do_token, do_head;
   int64_t dq_batch, dq_token, dq_head, dk_batch, dk_token, dk_head, dv_batch, dv_token, dv_head;
   float scale, scale_log2;
-  int kv_tiles;    // key tiles of a head
-  int sink_tiles;  // of them, tiles with a sink key; 0: nothing to join
+  int sink_tiles;  // key tiles with a sink key; 0: nothing to join
   int far_tiles;   // query tiles of a far piece (see kv_piece)
   int far_pieces;  // far pieces of a sink tile
   int kv_items, items;     // items [0, kv_items): key tiles, then query tiles
@@ -149,7 +149,7 @@ struct GradShared {
   uint64_t a_cleared;      // the storing warps' parts of it
   uint64_t b_full[kGradB], b_empty[kGradB];
   uint64_t st_full[2], st_empty[2];  // row statistics (key tiles)
-  uint64_t s_full[2], dp_full;       // key tiles use s_full[0] alone
+  uint64_t s_full, dp_full;          // S of key tiles; dP
   uint64_t q_s_full[2];              // the two S buffers of query tiles
   uint64_t p_ready, ds_ready;
   uint64_t sum_full[2], sum_free[2];  // dV; dK or dQ
@@ -186,7 +186,7 @@ __device__ __forceinline__ void grad_init(GradShared& sh) {
   init(sh.b_empty, kGradB, 1);
   init(sh.st_full, 2, 1);
   init(sh.st_empty, 2, kGradEwWarps);
-  init(sh.s_full, 2, 1);
+  init(&sh.s_full, 1, 1);
   init(&sh.dp_full, 1, 1);
   init(sh.q_s_full, 2, 1);
   init(&sh.p_ready, 1, kGradEwWarps);
@@ -551,7 +551,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
       ok = wait(&sh.own_full[0], op) && wait(&sh.a_full[a.slot], a.parity);
       if (!ok) break;
       mma_rows<D>(tmem + C::S, own0, rows_of(G::RING_A, a.slot), IDESC_S);
-      commit(&sh.s_full[0]);
+      commit(&sh.s_full);
       if (n == 1) commit(&sh.own_empty[0]);
       ok = wait(&sh.own_full[1], op) && wait(&sh.b_full[b.slot], b.parity);
       if (!ok) break;
@@ -575,7 +575,7 @@ __device__ __forceinline__ void grad_mma(const GradArgs& args, GradShared& sh, u
           ok = wait(&sh.a_full[a.slot], a.parity);
           if (!ok) break;
           mma_rows<D>(tmem + C::S, own0, rows_of(G::RING_A, a.slot), IDESC_S);
-          commit(&sh.s_full[0]);
+          commit(&sh.s_full);
           if (j + 2 == n) commit(&sh.own_empty[0]);
         }
         ok = wait(&sh.ds_ready, cnt & 1u);
@@ -740,7 +740,7 @@ struct GradEw {
       const int c_hi = (min(tok_hi, tb) - ta + 1) * g.g - wg * 64;
       const uint32_t see[2] = {bits_below(c_hi, 0) & ~bits_below(c_lo, 0),
                                bits_below(c_hi, 1) & ~bits_below(c_lo, 1)};
-      if (!wait(&sh.st_full[st.slot], st.parity) || !wait(&sh.s_full[0], cnt & 1u)) return;
+      if (!wait(&sh.st_full[st.slot], st.parity) || !wait(&sh.s_full, cnt & 1u)) return;
       if (masked && __all_sync(0xffffffffu, (see[0] | see[1]) == 0u)) {
         // no key of this warp is seen by its rows (behind the window of a
         // tile whose sinks are): P and dS are 0
@@ -1147,7 +1147,6 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   a.wide_dkv = rows_on_32(gp.dk) && rows_on_32(gp.dv);
   a.scale = p.scale;
   a.scale_log2 = p.scale * 1.4426950408889634f;
-  a.kv_tiles = pl.kv_tiles;
   a.sink_tiles = pl.sink_tiles;
   a.far_tiles = pl.far_tiles;
   a.far_pieces = pl.far_pieces;
