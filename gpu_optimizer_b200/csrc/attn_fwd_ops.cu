@@ -448,6 +448,19 @@ __device__ __forceinline__ void fwd_regs_inc() {
 __device__ __forceinline__ void fwd_barrier(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
+// The same, and whether all four warps say so.  A warp that leaves its work
+// (done, or a wait gave up) votes no once: a warp whose last wait ended in time
+// is not left at the barrier for good by one whose wait did not.
+__device__ __forceinline__ bool fwd_vote(int id, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(yes ? 1u : 0u), "r"(id)
+      : "memory");
+  return all != 0;
+}
 
 // Joins the parts [c0, c1] of a unit with few rows (16 at most), in their
 // order and against a running maximum.  A thread has every nx-th vector of four
@@ -1079,7 +1092,7 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
         }
       }
       __threadfence();
-      fwd_barrier(1 + t);
+      if (!fwd_vote(1 + t, true)) return;
       if (row == 0) {
         unsigned int* cnt = args.arrived + static_cast<int64_t>(s.unit) * TILES + t;
         const unsigned int before = atomicAdd(cnt, 1u);
@@ -1173,6 +1186,7 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
       }
     }
   }
+  if (STREAM) fwd_vote(1 + t, false);
 }
 
 template <typename T, int FMT, int D, bool PAGED, bool STREAM, int TILES, bool UNSEEN>
