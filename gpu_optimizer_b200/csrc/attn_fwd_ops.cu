@@ -1381,7 +1381,8 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
   a.spans = fwd_spans(g);
   // Two Q tiles and the staging tile of D = 128 leave room for four slots
   // (a third V slot in the staging tile's place measured the same).
-  a.k_stages = a.v_stages = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
+  constexpr int STAGES = TILES == 1 || D == 64 ? kFwdMaxStages : 2;
+  a.k_stages = a.v_stages = STAGES;
   a.wide = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0 && p.o_batch % 16 == 0 &&
            p.o_token % 16 == 0 && p.o_head % 16 == 0;
   a.err = c.err;
@@ -1398,9 +1399,9 @@ gpo_status run_fwd(const AttnProblem& p, const LaunchCtx& c) {
     ctas = sms;
   }
   auto kern = attn_fwd_kernel<T, FMT, D, PAGED, STREAM, TILES, UNSEEN>;
-  const uint32_t dyn =
-      (TILES * 128u + static_cast<uint32_t>(a.k_stages + a.v_stages) * kOpsBN +
-       (TILES == 2 ? 128u : 0u)) * D * 2u + 1024u;
+  constexpr uint32_t dyn =
+      (TILES * 128u + 2u * STAGES * kOpsBN + (TILES == 2 ? 128u : 0u)) * D * 2u + 1024u;
+  static_assert(dyn + sizeof(FwdShared) > kOpsAloneBytes, "two CTAs fit an SM");
   gpo_status s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
   return launch_in_order(kern, static_cast<unsigned>(ctas), 128 + 128 * TILES, dyn, c.stream, mq,

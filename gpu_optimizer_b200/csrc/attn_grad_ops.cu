@@ -1167,6 +1167,7 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   auto kern = attn_has_unseen(g) ? attn_grad_kernel<T, FMT, D, true>
                                  : attn_grad_kernel<T, FMT, D, false>;
   constexpr uint32_t dyn = GradGeom<D>::BYTES;
+  static_assert(dyn > kOpsAloneBytes, "two CTAs fit an SM");
   s = ensure_smem_attr(reinterpret_cast<const void*>(kern), dyn);
   if (s != GPO_OK) return s;
   s = launch_in_order(kern, static_cast<unsigned>(std::min(a.items, sms)), kGradThreads, dyn,

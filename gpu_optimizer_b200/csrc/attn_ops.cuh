@@ -214,6 +214,13 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// A CTA of these kernels asks for all of its SM's TMEM, and one that has
+// started early (see below) keeps it while it waits for the kernel before: on
+// an SM where that kernel's CTA had not got its own yet, both would wait for
+// good.  They never share an SM, as each takes more than half of its shared
+// memory (228 KB, 1 KB of every CTA reserved).
+constexpr uint32_t kOpsAloneBytes = 113u * 1024u;  // a CTA's own, more than
+
 // Launch order within a stream: a kernel launched by launch_in_order may
 // start (barriers, TMEM, descriptors) while the kernel before it still runs,
 // and touches global memory only behind wait_for_previous.
