@@ -110,6 +110,11 @@ def _workspace(args: type) -> tuple:
                           ctypes.c_char_p, ctypes.c_size_t]
 
 
+def _kernel(args: type) -> tuple:
+    """Signature of an operator's kernel name: (args, name, name_cap)."""
+    return ctypes.c_int, [ctypes.POINTER(args), ctypes.c_char_p, ctypes.c_size_t]
+
+
 # Every symbol include/gpo.h declares, with its ctypes signature.
 SIGNATURES = {
     "gpo_abi_version": (ctypes.c_int, []),
@@ -125,8 +130,10 @@ SIGNATURES = {
                                                  ctypes.c_int32, ctypes.c_void_p]),
     "gpo_window_attention": _operator(GpoWindowArgs),
     "gpo_window_attention_grad": _operator(GpoWindowArgs),
+    "gpo_window_kernel": _kernel(GpoWindowArgs),
     "gpo_window_workspace": _workspace(GpoWindowArgs),
     "gpo_paged_attention": _operator(GpoPagedArgs),
+    "gpo_paged_kernel": _kernel(GpoPagedArgs),
     "gpo_paged_workspace": _workspace(GpoPagedArgs),
     "gpo_cache_append": _operator(GpoPagedArgs),
     "gpo_destroy": (None, [ctypes.c_void_p]),

@@ -34,6 +34,7 @@ anything is launched; a launch that fails raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import ctypes
 import importlib
 
 import torch
@@ -189,10 +190,29 @@ OPERATOR_INPUTS = {
     "attention_paged": ("q", "k_pages", "v_pages", "page_table", "q_start", "kv_len"),
     "cache_append": ("k", "v", "k_pages", "v_pages", "page_table", "q_start", "kv_len"),
 }
-_KERNELS = {"attention_window": "attn_fwd_kernel<dense>",
-            "attention_window_grad": "attn_grad_kernel",
-            "attention_paged": "attn_fwd_kernel<paged>",
-            "cache_append": "cache_append_kernel"}
+_KERNELS = {"attention_window_grad": "attn_grad_kernel", "cache_append": "cache_append_kernel"}
+
+
+def kernel_name(task: str, shape, config: dict, tokens: int = 0) -> str:
+    """The kernel instance that a call launches, as the library chooses it;
+    ``tokens``: the rows of q of a paged call."""
+    if task in _KERNELS:
+        return _KERNELS[task]
+    dtype = _lib.DTYPE_IDS[str(config.get("dtype", "bfloat16"))]
+    mask = (int(config.get("window", 0)), int(config.get("sinks", 0)), 0.0, 0)
+    if task == "attention_window":
+        b, q_len, kv_len, hq, hk, dim = shape
+        query, args = "gpo_window_kernel", _lib.GpoWindowArgs(dtype, dim, hq, hk, b, q_len, kv_len,
+                                                              *mask)
+    else:
+        seqs, max_q, page_size, hq, hk, dim = shape
+        query, args = "gpo_paged_kernel", _lib.GpoPagedArgs(dtype, dim, hq, hk, seqs, tokens, max_q,
+                                                            0, page_size, 0, 0, *mask)
+    name = ctypes.create_string_buffer(256)
+    rc = getattr(_lib.load(), query)(args, name, 256)
+    if rc != _lib.OK:
+        raise KernelBuildError(f"{task}: {name.value.decode()}")
+    return name.value.decode()
 
 
 def operator_call(task: str, shape, config: dict, inputs):
@@ -244,4 +264,5 @@ def operator_call(task: str, shape, config: dict, inputs):
             def fn():
                 plan.append(*inputs)
                 return t["k_pages"], t["v_pages"]
-    return fn, f"b200 {_KERNELS[task]}", {"kernel": _KERNELS[task], **config}
+    kernel = kernel_name(task, shape, config, first.shape[0])
+    return fn, f"b200 {kernel}", {"kernel": kernel, **config}

@@ -1432,6 +1432,16 @@ uint64_t attn_paged_workspace(const AttnProblem& p) {
          2u * kFwdMaxCtas * static_cast<uint64_t>(fwd_part_floats(fwd_part_rows(g), p.dim)) * 4u;
 }
 
+std::string attn_forward_name(const AttnProblem& p) {
+  const AttnGeom& g = p.geom;
+  std::string s = std::string("attn_fwd_kernel<") + (p.dtype == GPO_BFLOAT16 ? "bf16" : "f16") +
+                  ",D=" + std::to_string(p.dim) + (p.paged ? ",paged" : ",dense") +
+                  ",tiles=" + std::to_string(fwd_tiles(g));
+  if (p.paged && fwd_is_cut(g)) s += ",cut";
+  if (!p.paged && attn_has_unseen(g)) s += ",unseen";
+  return s + ">";
+}
+
 gpo_status launch_attn_forward(const AttnProblem& p, const LaunchCtx& c) {
   if (p.dtype == GPO_BFLOAT16)
     return p.dim == 128 ? run_fwd_form<__nv_bfloat16, 1, 128>(p, c)

@@ -12,6 +12,8 @@
 // (p - j < window or j < sinks).
 #pragma once
 
+#include <string>
+
 #include "gpo_common.cuh"
 #include "gpo_internal.h"
 
@@ -354,6 +356,7 @@ struct AttnGradProblem {
 uint64_t attn_grad_workspace(const AttnProblem& p);
 gpo_status launch_attn_grad(const AttnProblem& p, const AttnGradProblem& gp, const LaunchCtx& c);
 uint64_t attn_paged_workspace(const AttnProblem& p);
+std::string attn_forward_name(const AttnProblem& p);
 gpo_status launch_attn_forward(const AttnProblem& p, const LaunchCtx& c);
 gpo_status launch_cache_append(const AttnProblem& p, const LaunchCtx& c);
 

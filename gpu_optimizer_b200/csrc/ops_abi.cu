@@ -233,6 +233,19 @@ gpo_status gpo_window_attention(const gpo_window_args* a, void* stream, char* lo
   }
 }
 
+gpo_status gpo_window_kernel(const gpo_window_args* a, char* name, size_t cap) {
+  if (!a) return GPO_BAD_ARGS;
+  try {
+    AttnProblem p{};
+    Refusal r;
+    if (!dense_problem(*a, false, p, r)) return refuse(r, name, cap);
+    write_log(name, cap, attn_forward_name(p));
+    return GPO_OK;
+  } catch (...) {
+    return GPO_INTERNAL;
+  }
+}
+
 gpo_status gpo_window_workspace(const gpo_window_args* a, uint64_t* bytes, char* log,
                                 size_t cap) {
   if (!a || !bytes) return GPO_BAD_ARGS;
@@ -298,6 +311,19 @@ gpo_status gpo_window_attention_grad(const gpo_window_args* a, void* stream, cha
       return refuse(r, log, cap);
     }
     return guarded(stream, log, cap, [&](LaunchCtx& c) { return launch_attn_grad(p, gp, c); });
+  } catch (...) {
+    return GPO_INTERNAL;
+  }
+}
+
+gpo_status gpo_paged_kernel(const gpo_paged_args* a, char* name, size_t cap) {
+  if (!a) return GPO_BAD_ARGS;
+  try {
+    AttnProblem p{};
+    Refusal r;
+    if (!paged_problem(*a, false, true, p, r)) return refuse(r, name, cap);
+    write_log(name, cap, attn_forward_name(p));
+    return GPO_OK;
   } catch (...) {
     return GPO_INTERNAL;
   }

@@ -283,6 +283,10 @@ GPO_API gpo_status gpo_window_attention(const gpo_window_args* args, void* strea
  * vanishes; scale the loss). */
 GPO_API gpo_status gpo_window_attention_grad(const gpo_window_args* args, void* stream, char* log,
                                              size_t log_cap);
+/* Name of the kernel instance that gpo_window_attention launches for `args`
+ * (its pointers are not looked at), as gpo_query gives it for a task; the
+ * reason of a refusal in its place. */
+GPO_API gpo_status gpo_window_kernel(const gpo_window_args* args, char* name, size_t name_cap);
 /* Bytes of workspace that gpo_window_attention_grad needs for `args` (its
  * pointers are not looked at). */
 GPO_API gpo_status gpo_window_workspace(const gpo_window_args* args, uint64_t* bytes, char* log,
@@ -296,6 +300,7 @@ GPO_API gpo_status gpo_window_workspace(const gpo_window_args* args, uint64_t* b
  * and where a key of it is seen, that is reported in the same way. */
 GPO_API gpo_status gpo_paged_attention(const gpo_paged_args* args, void* stream, char* log,
                                        size_t log_cap);
+GPO_API gpo_status gpo_paged_kernel(const gpo_paged_args* args, char* name, size_t name_cap);
 GPO_API gpo_status gpo_paged_workspace(const gpo_paged_args* args, uint64_t* bytes, char* log,
                                        size_t log_cap);
 /* Write the new tokens' rows k_new, v_new to the last slots of their
