@@ -62,6 +62,7 @@ struct GradArgs {
   int sink_tiles;  // key tiles with a sink key; 0: nothing to join
   int far_tiles;   // query tiles of a far piece (see kv_piece)
   int far_pieces;  // far pieces of a sink tile
+  int blind;               // first tokens, which see no key
   int kv_items, items;     // items [0, kv_items): key tiles, then query tiles
   unsigned int* next;      // counter of items, zeroed by the statistics kernel
   bool wide_dq, wide_dkv;  // rows on 32 bytes
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
   for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += RPW) {
     const int r = r0 + lane / LPR;
     const int token = tile * g.tpt + r / g.g, head = h * g.g + r % g.g;
-    const bool live = r < g.tpt * g.g && token < g.q_len;
+    const bool live = r < g.tpt * g.g && token < g.q_len && token >= a.blind;
     float s = 0.f, l = 0.f;
     if (live) {
       if (lane % LPR == 0)
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(256) attn_grad_stats_kernel(const GradArgs a) 
     if (lane % LPR == 0) {
       float nl = -INFINITY;  // no query in this row: P is 0
       if (live) {
-        // a row that saw no key (L = -inf) has P = 0 everywhere, too
+        // a row whose scores were all -inf has P = 0 everywhere, too
         nl = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
       }
       st[r] = nl;
@@ -405,7 +406,9 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
   auto wait = [&](const uint64_t* bar, uint32_t parity) {
     return mbar_wait(smem_u32(bar), parity, abort_flag, err, kErrWaitProducer);
   };
-  // 128 keys from `row`, or the rows of a query tile
+  // 128 keys from `row`, or the rows of a query tile.  Tokens that see no key
+  // may hold anything: the maps of Q and dO begin behind them, and what a copy
+  // asks for in front of a map arrives as zeros.
   uint32_t raw = 0, raw_parity = 0;  // bit s: slot s's last copy ends at a_raw; its parity
   auto load_keys = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int h, int row, int b) {
     mbar_arrive_expect_tx(smem_u32(bar), G::TILE);
@@ -418,7 +421,7 @@ __device__ __forceinline__ void grad_producer(const GradArgs& args, GradShared& 
     mbar_arrive_expect_tx(smem_u32(bar), rows_bytes);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
-      tma_load_5d(dst + c * 128 * 128, m, smem_u32(bar), c * 64, 0, h, token, b);
+      tma_load_5d(dst + c * 128 * 128, m, smem_u32(bar), c * 64, 0, h, token - args.blind, b);
   };
   bool ok = true;
   int own = 0, issued = 0, stats = 0;
@@ -1116,8 +1119,15 @@ template <typename T, int FMT, int D>
 gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const LaunchCtx& c) {
   const AttnGeom& g = p.geom;
   CUtensorMap mq, mdo, mk, mv;
-  if (!encode_rows_map(&mq, p.dtype, p.q, D, g.g, g.tpt) ||
-      !encode_rows_map(&mdo, p.dtype, gp.dout, D, g.g, g.tpt) ||
+  // (kv_len = 0: nothing is loaded, and the maps stay whole)
+  const int blind = g.kv_len > 0 ? std::max(0, g.q_len - g.kv_len) : 0;
+  auto seeing = [&](HeadsView t) {
+    t.ptr = static_cast<const char*>(t.ptr) + blind * t.s_token * 2;
+    t.tokens -= blind;
+    return t;
+  };
+  if (!encode_rows_map(&mq, p.dtype, seeing(p.q), D, g.g, g.tpt) ||
+      !encode_rows_map(&mdo, p.dtype, seeing(gp.dout), D, g.g, g.tpt) ||
       !encode_keys_map(&mk, p.dtype, p.k, D, 128) || !encode_keys_map(&mv, p.dtype, p.v, D, 128))
     return GPO_BAD_ARGS;
   const GradPlan pl = grad_plan(g, D);
@@ -1150,6 +1160,7 @@ gpo_status run_grad(const AttnProblem& p, const AttnGradProblem& gp, const Launc
   a.sink_tiles = pl.sink_tiles;
   a.far_tiles = pl.far_tiles;
   a.far_pieces = pl.far_pieces;
+  a.blind = blind;
   a.err = c.err;
   const int64_t heads = static_cast<int64_t>(g.batch) * g.heads_kv;
   const int64_t q_items = heads * g.tiles;

@@ -210,9 +210,12 @@ GPO_API gpo_status gpo_reduction_sum_noalloc(const float* x, int64_t n, float* o
  * Mask of all of them: token i of a sequence with q_len new tokens and
  * kv_len keys stands at position p = i + kv_len - q_len and sees key j iff
  * j <= p and (p - j < window or j < sinks).  A row that sees no key gives 0
- * and a log-sum-exp of -inf.  What a masked place holds (NaN and infinities
- * included) does not reach the scores; the values that a masked key weighs
- * with 0 have to be finite wherever another row of the sequence sees it.
+ * and a log-sum-exp of -inf.  Keys that no row of the sequence sees, and rows
+ * that see no key, may hold anything (NaN and infinities included), slots
+ * behind the last key too.  What a masked key of a row holds never reaches its
+ * scores; where another row sees that key, its values (in the gradient: its
+ * K, and q and dout of the rows) have to be finite, as a weight of 0 takes
+ * them into the sum.
  *
  * Query head h reads kv head h / (heads_q / heads_kv).  Element types:
  * GPO_FLOAT16 or GPO_BFLOAT16, fp32 scores, statistics and sums.

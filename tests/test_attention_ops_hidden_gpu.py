@@ -122,3 +122,33 @@ def test_window_gradient_hidden_keys_may_hold_anything(case, dtype, which):
     for a, w in zip(got, want):
         assert torch.isfinite(w).all() and torch.equal(a, w)
     assert not got[1][:, keys].any() and not got[2][:, keys].any()
+
+
+@pytest.mark.parametrize("case", [
+    (1, 300, 100, 4, 2, 64, None, 0),
+    (2, 513, 130, 3, 1, 128, 40, 4),     # tokens without a key end inside a tile
+    (1, 1500, 700, 8, 8, 128, 200, 0),
+    (1, 260, 4, 16, 2, 64, 2, 1),
+], ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "f16"])
+@pytest.mark.parametrize("which", ["q", "dout"])
+def test_window_tokens_without_a_key_may_hold_anything(case, dtype, which):
+    """More queries than keys: the first ones see nothing, give nothing to dK
+    and dV, and their own gradient is 0."""
+    b, q_len, kv_len, hq, hk, d, window, sinks = case
+    mask = {"window": window, "sinks": sinks}
+    q, k, v = heads(b, q_len, kv_len, hq, hk, d, dtype, seed=kv_len)
+    dout = normal(b, q_len, hq, d, seed=42, dtype=dtype)
+    out, lse = ops.window_attention_forward(q, k, v, **mask)
+    want = ops.window_attention_backward(dout, q, k, v, out, lse, **mask)
+    blind = q_len - kv_len
+    t = q if which == "q" else dout
+    t[:, :blind] = math.nan
+    t[:, :blind:3] = -math.inf
+    again, lse2 = ops.window_attention_forward(q, k, v, **mask)
+    assert torch.equal(again, out) and torch.equal(lse2, lse)
+    got = ops.window_attention_backward(dout, q, k, v, out, lse, **mask)
+    check_device_status()
+    for a, w in zip(got, want):
+        assert torch.isfinite(w).all() and torch.equal(a, w)
+    assert not got[0][:, :blind].any()
