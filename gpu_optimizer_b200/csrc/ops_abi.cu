@@ -56,6 +56,13 @@ bool check_heads(const gpo_heads& t, const char* name, int64_t batch, int64_t to
   return true;
 }
 
+// An array of 32-bit values (null is the caller's matter).
+bool check_array(const void* p, const char* name, Refusal& r) {
+  if (reinterpret_cast<uintptr_t>(p) & 3u)
+    return r.no(GPO_BAD_ARGS, std::string(name) + " is not 4-byte aligned");
+  return true;
+}
+
 // Strides an output must not fold onto itself.
 bool check_written(const gpo_heads& t, const char* name, int64_t batch, int64_t tokens, int heads,
                    int dim, Refusal& r) {
@@ -166,6 +173,9 @@ bool paged_problem(const gpo_paged_args& a, bool pointers, bool attention, AttnP
   if (!pointers || a.num_seqs == 0 || a.tokens == 0) return true;
   if (!a.q_start || !a.kv_len || (a.table_width > 0 && !a.page_table))
     return r.no(GPO_BAD_ARGS, "page_table, q_start or kv_len is null");
+  if (!check_array(a.page_table, "page_table", r) || !check_array(a.q_start, "q_start", r) ||
+      !check_array(a.kv_len, "kv_len", r) || !check_array(a.lse, "lse", r))
+    return false;
   if (a.num_pages > 0) {
     if (!check_written(a.k_pages, "k_pages", a.num_pages, a.page_size, a.heads_kv, a.head_dim, r) ||
         !check_written(a.v_pages, "v_pages", a.num_pages, a.page_size, a.heads_kv, a.head_dim, r))
@@ -220,7 +230,8 @@ gpo_status gpo_window_attention(const gpo_window_args* a, void* stream, char* lo
     Refusal r;
     if (!dense_problem(*a, true, p, r)) return refuse(r, log, cap);
     if (a->batch == 0 || a->q_len == 0) return GPO_OK;
-    if (!check_written(a->out, "out", a->batch, a->q_len, a->heads_q, a->head_dim, r))
+    if (!check_written(a->out, "out", a->batch, a->q_len, a->heads_q, a->head_dim, r) ||
+        !check_array(a->lse, "lse", r))
       return refuse(r, log, cap);
     p.out = a->out.ptr;
     p.o_batch = a->out.stride_batch;
@@ -276,7 +287,8 @@ gpo_status gpo_window_attention_grad(const gpo_window_args* a, void* stream, cha
     if (q > 0) {
       if (!check_heads(a->out, "out", b, q, a->heads_q, r) ||
           !check_heads(a->dout, "dout", b, q, a->heads_q, r) ||
-          !check_written(a->dq, "dq", b, q, a->heads_q, a->head_dim, r))
+          !check_written(a->dq, "dq", b, q, a->heads_q, a->head_dim, r) ||
+          !check_array(a->lse, "lse", r))
         return refuse(r, log, cap);
       if (!a->lse) {
         r.no(GPO_BAD_ARGS, "lse is null");

@@ -10,7 +10,7 @@ import torch
 from gpu_optimizer_b200 import _lib
 from gpu_optimizer_b200 import attention_ops as ops
 from gpu_optimizer_b200.runner import KernelBuildError
-from test_attention_ops import call, paged, window
+from test_attention_ops import call, heads, paged, window
 
 PLAN = dict(heads_q=4, heads_kv=2, head_dim=64, page_size=16, max_seqs=2, max_q=4,
             dtype=torch.bfloat16, device="cuda:0")
@@ -54,3 +54,23 @@ def test_plans_may_allow_more_tokens_than_a_call_has():
     for bad in ({"max_seqs": 65536}, {"max_q": (1 << 30) + 1}, {"max_q": 1 << 62, "max_seqs": 4}):
         with pytest.raises(KernelBuildError, match="num_seqs"):
             ops.PagedAttention(**{**PLAN, **bad})
+
+
+def test_pointers_off_their_types_grid_are_refused():
+    """A misaligned address is a fault on the device."""
+    q = heads(4096, 2048, 256, 64)
+    kv = heads(4096, 1024, 128, 64)
+    dense = dict(q=q, k=kv, v=kv, out=q, lse=4098)
+    rc, log = call("gpo_window_attention", window(**dense), None)
+    assert rc == _lib.BAD_ARGS and "lse is not 4-byte aligned" in log
+    grads = dict(dense, dout=q, dq=q, dk=kv, dv=kv)
+    rc, log = call("gpo_window_attention_grad", window(**grads), None)
+    assert rc == _lib.BAD_ARGS and "lse is not 4-byte aligned" in log
+    pages = dict(k_pages=heads(4096, 2048, 128, 64), v_pages=heads(4096, 2048, 128, 64),
+                 q=heads(4096, 0, 256, 64), out=heads(4096, 0, 256, 64), page_table=64, q_start=64,
+                 kv_len=64, lse=64, k_new=heads(4096, 0, 128, 64), v_new=heads(4096, 0, 128, 64))
+    for name in ("page_table", "q_start", "kv_len", "lse"):
+        rc, log = call("gpo_paged_attention", paged(**{**pages, name: 66}), None)
+        assert rc == _lib.BAD_ARGS and f"{name} is not 4-byte aligned" in log, log
+    rc, log = call("gpo_cache_append", paged(**{**pages, "kv_len": 65}), None)
+    assert rc == _lib.BAD_ARGS and "kv_len is not 4-byte aligned" in log
