@@ -177,9 +177,13 @@ bool paged_problem(const gpo_paged_args& a, bool pointers, bool attention, AttnP
       !check_array(a.kv_len, "kv_len", r) || !check_array(a.lse, "lse", r))
     return false;
   if (a.num_pages > 0) {
-    if (!check_written(a.k_pages, "k_pages", a.num_pages, a.page_size, a.heads_kv, a.head_dim, r) ||
-        !check_written(a.v_pages, "v_pages", a.num_pages, a.page_size, a.heads_kv, a.head_dim, r))
-      return false;
+    for (int i = 0; i < 2; ++i) {
+      const gpo_heads& t = i ? a.v_pages : a.k_pages;
+      const char* name = i ? "v_pages" : "k_pages";
+      if (attention ? !check_heads(t, name, a.num_pages, a.page_size, a.heads_kv, r)
+                    : !check_written(t, name, a.num_pages, a.page_size, a.heads_kv, a.head_dim, r))
+        return false;
+    }
     p.k = view(a.k_pages, a.num_pages, a.page_size, a.heads_kv);
     p.v = view(a.v_pages, a.num_pages, a.page_size, a.heads_kv);
   }

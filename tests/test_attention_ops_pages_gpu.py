@@ -6,6 +6,7 @@ import torch
 
 from gpu_optimizer_b200 import attention_ops as ops
 from gpu_optimizer_b200 import _lib
+from gpu_optimizer_b200.runner import KernelBuildError
 from test_attention_ops_gpu import normal
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +110,20 @@ def test_attend_reports_seen_pages_outside_the_cache(max_q, window, slot, report
         out = p.attend(q, kp, vp, table, ints(0, m), ints(n))
         assert flags() == (0x20 if reported else 0)
         assert torch.isfinite(out).all() and torch.equal(out, want) != reported
+
+
+def test_attend_reads_a_cache_whose_heads_are_one():
+    """A cache with one kv head, expanded: read in place by attend, refused by
+    append, which would write its rows over each other."""
+    p = plan(4, 4, 64, 16, 1, 2)
+    k = normal(5, 16, 1, 64, seed=57, dtype=torch.bfloat16)
+    v = normal(5, 16, 1, 64, seed=58, dtype=torch.bfloat16)
+    q = normal(2, 4, 64, seed=59, dtype=torch.bfloat16)
+    where = ints(4, 2, 0, 1, 3)[None], ints(0, 2), ints(70)
+    flags()
+    got = p.attend(q, k.expand(-1, -1, 4, -1), v.expand(-1, -1, 4, -1), *where)
+    want = p.attend(q, k.repeat(1, 1, 4, 1), v.repeat(1, 1, 4, 1), *where)
+    assert flags() == 0 and torch.equal(got, want)
+    with pytest.raises(KernelBuildError, match="rows overlap"):
+        p.append(normal(2, 4, 64, seed=60, dtype=torch.bfloat16), q, k.expand(-1, -1, 4, -1),
+                 v.expand(-1, -1, 4, -1), *where)
