@@ -110,6 +110,17 @@ gpo_status launch_ctx(void* stream, LaunchCtx* out) {
     cudaGetLastError();
     return GPO_NO_DEVICE;
   }
+  // Tensor maps are encoded by a driver call, which needs the device's context
+  // to be current in the calling thread; the runtime's own calls see to that
+  // only when they come to one that uses the device.
+  thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) {
+      cudaGetLastError();
+      return GPO_NO_DEVICE;
+    }
+    bound = dev;
+  }
   DeviceState* ds = nullptr;
   const gpo_status s = device_state(dev, &ds);
   if (s != GPO_OK) return s;
@@ -237,15 +248,9 @@ gpo_status gpo_query(const gpo_module* mod, gpo_resources* res) {
 
 gpo_status gpo_launch(gpo_module* mod, const gpo_args* args, void* stream) {
   if (!mod || !args) return GPO_BAD_ARGS;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) {
-    cudaGetLastError();
-    return GPO_NO_DEVICE;
-  }
-  gpo::DeviceState* ds = nullptr;
-  gpo_status s = gpo::device_state(dev, &ds);
+  gpo::LaunchCtx ctx;
+  const gpo_status s = gpo::launch_ctx(stream, &ctx);
   if (s != GPO_OK) return s;
-  gpo::LaunchCtx ctx{static_cast<cudaStream_t>(stream), ds->err, dev, ds->sm_count};
   gpo_args a = *args;
   if (a.scale == 0.f) a.scale = 0.7071f;  // benchmarks/fused_elementwise/task.py:19
   if (a.eps == 0.f) a.eps = 1e-5f;        // benchmarks/layernorm/task.py:15
