@@ -12,6 +12,8 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
+#include <map>
+#include <mutex>
 #include <string>
 
 #include "gpo.h"
@@ -233,6 +235,18 @@ std::tuple<Tensor, Tensor, Tensor> window_backward(
 }
 
 // ------------------------------------------------------------------- paged
+// The stream of a device that plans are made on: one for all, so that a plan
+// takes up the memory that another has given back, and not one of the pool,
+// where other work may be queued.
+c10::cuda::CUDAStream plan_stream(c10::DeviceIndex device) {
+  static std::mutex mutex;
+  static std::map<c10::DeviceIndex, cudaStream_t> streams;
+  const std::lock_guard<std::mutex> lock(mutex);
+  cudaStream_t& s = streams[device];
+  if (!s) C10_CUDA_CHECK(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking));
+  return c10::cuda::getStreamFromExternal(s, device);
+}
+
 constexpr int64_t kMostTokens = 1ll << 30;  // of a call (gpo.h)
 
 struct Plan {
@@ -268,8 +282,8 @@ struct Plan {
   }
 
   // The workspace is zero before the plan is handed out, whichever stream
-  // calls it first.  It is made on a stream of its own, which alone is waited
-  // for; in a capture the zeroing becomes a part of the graph.
+  // calls it first.  It is made on the plans' own stream, which alone is
+  // waited for; in a capture the zeroing becomes a part of the graph.
   void make_workspace() {
     const auto bytes = static_cast<int64_t>(args.workspace_bytes);
     const auto options = at::TensorOptions().dtype(at::kByte).device(device);
@@ -278,7 +292,7 @@ struct Plan {
       work = at::zeros({bytes}, options);
       return;
     }
-    const auto own = c10::cuda::getStreamFromPool(false, device.index());
+    const auto own = plan_stream(device.index());
     const c10::cuda::CUDAStreamGuard guard(own);
     work = at::zeros({bytes}, options);
     own.synchronize();

@@ -90,3 +90,15 @@ def test_plan_made_in_a_capture():
         torch.cuda.synchronize()
         assert torch.equal(held, want)
     check_device_status()
+
+
+def test_plans_take_up_the_memory_of_those_before():
+    c = problem()
+    for _ in range(2):
+        attend(plan_for(c, *HEADS, torch.bfloat16), c)
+        torch.cuda.synchronize()
+    held = torch.cuda.memory_reserved()
+    for _ in range(40):
+        attend(plan_for(c, *HEADS, torch.bfloat16), c)
+        torch.cuda.synchronize()
+    assert torch.cuda.memory_reserved() == held
