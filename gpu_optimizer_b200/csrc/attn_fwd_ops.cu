@@ -42,19 +42,21 @@
 // the CTAs' work, the joins met there (16 chunks of 512 over 2K: 231 -> 249 us).
 //
 // What bounds it, bf16, D 128, 32 heads over 8 (B200, 6.55 TB/s and 1650
-// TFLOP/s measured):
-//   prefill of 8192, window 1024   155 us, 834 TFLOP/s of the visible pairs;
-//                                  the tensor pipe and the exp2 unit are both
-//                                  busy 53 % of the time: a step of a pair of
-//                                  tiles (2.1 us) is the chain S -> maximum ->
-//                                  exp2 -> P -> PV, twice, half overlapped
-//   4 x 4096 causal                495 us, 1110 TFLOP/s, as above
-//   64 single tokens, 0.8K..8K     191 us, 0.91 of the copy rate: HBM
-//   2 single tokens, 4 kv heads,   97 us, 0.84 of it: HBM, and SMs that end up
-//     128K                         to a third before the last
-//   one token over 777             11 us: launch, a chain of dependent loads
-//                                  (length, page, K, V) and the join
-//   4 chunks of 512 over 8K        234 us, 1030 TFLOP/s; as the prefill
+// TFLOP/s measured; under sustained load with inputs that change from pass to
+// pass, in brackets a short loop over the same inputs, as are the figures
+// beside the rules and steps below):
+//   prefill of 8192, window 1024   173 us (151), 747 TFLOP/s of the visible
+//                                  pairs; the tensor pipe and the exp2 unit are
+//                                  both busy 53 % of the time: a step of a pair
+//                                  of tiles (2.1 us) is the chain S -> maximum
+//                                  -> exp2 -> P -> PV, twice, half overlapped
+//   4 x 4096 causal                534 us, 1030 TFLOP/s, as above
+//   64 single tokens, 0.8K..8K     218 us (192), 0.80 of the copy rate: HBM
+//   2 single tokens, 4 kv heads,   101 us (97), 0.80 of it: HBM, and SMs that
+//     128K                         end up to a quarter before the last
+//   one token over 777             11.3 us (11.0): launch, a chain of dependent
+//                                  loads (length, page, K, V) and the join
+//   4 chunks of 512 over 8K        277 us (235), 865 TFLOP/s; as the prefill
 #include <algorithm>
 
 #include "attn_ops.cuh"
@@ -1125,7 +1127,10 @@ __device__ __forceinline__ void fwd_softmax(const FwdArgs& args, FwdShared& sh, 
           return __ldcg(reinterpret_cast<const float4*>(part_of(c)) + base + r +
                         x * args.part_rows);
         };
-        // with two tiles a unit has two or three parts, few rows or many
+        // With two tiles the join of few rows spilled (4 chunks of 512 over 8K
+        // 235 -> 270..350 us): rows each take a thread there.  Units of two
+        // tiles have many rows and two or three parts, unless a plan that takes
+        // chunks is called for single tokens (see fwd_tiles).
         if (TILES == 1 && rows <= 16) {
           if constexpr (TILES == 1)
             fwd_join(row, rows, D / 4, c_first, c_last, load_ml, load, finish);
@@ -1324,7 +1329,11 @@ namespace {
 // more than two tiles: with fewer, a tile per CTA ends earlier.  One tile
 // against two, bf16, D 128, 32 heads over 8, window 1024: 1 x 512 tokens
 // 10.6 / 14.4 us, 1024 17.3 / 22.6, 2048 43.5 / 41.5, 8192 183 / 155; paged,
-// 4 chunks of 512 over 8K 293 / 247.
+// 4 chunks of 512 over 8K 293 / 247.  The host knows max_q, not the lengths: a
+// call for single tokens from a plan that takes chunks gets two tiles, one of
+// them empty (64 tokens over 0.8K..8K from a plan of max_q 1 / 512: 196 / 252
+// us; with a window of 1024 65 / 91; 256 over 0.2K..2K 238 / 317; 16 tokens 52
+// / 52).  A plan for each kind of step avoids it.
 int fwd_tiles(const AttnGeom& g) {
   int64_t tiles = static_cast<int64_t>(cdiv(g.q_len, g.tpt)) * g.batch;
   // paged: the rows of all sequences together fill no more than

@@ -163,8 +163,10 @@ __device__ __forceinline__ bool block_is_masked(const AttnGeom& g, const AttnSeq
 // 2^x of two values on the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by
 // a polynomial of least relative error on that interval (7.5e-5 of degree 3,
 // 2.6e-6 of degree 4; fitted by iteratively reweighted least squares), 2^n
-// multiplied in.  For values that are rounded to 16 bits next (degree 3:
-// bfloat16, 4: float16).  x below -126 gives 2^-126, NaN stays NaN.
+// multiplied in.  For P of the gradient (degree 3: bfloat16, 4: float16), which
+// reaches its sums rounded to 16 bits, by itself or as the factor of dS = P *
+// (dP - delta): dS takes over P's relative error, a 52nd (a 188th) of what its
+// own rounding may take.  x below -126 gives 2^-126, NaN stays NaN.
 template <int DEGREE>
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to integer

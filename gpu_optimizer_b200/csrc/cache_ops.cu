@@ -3,9 +3,9 @@
 // few tokens a launch.  One thread moves one 16-byte vector of a row of K
 // and of V; the token's sequence is found by a binary search of q_start,
 // whose values every thread of a block reads from the same cache lines.
-// 8 chunks of up to 1024 tokens (8 heads, D 128, 16 bits; 57 MB): 12.3 us, 4.6
+// 8 chunks of up to 1024 tokens (8 heads, D 128, 16 bits; 57 MB): 11.7 us, 4.8
 // TB/s, of which some 4 us are the launch and the chain of loads before the
-// copy; 64 single tokens: 3.8 us.  Two vectors per thread were slower (3.1 ->
+// copy; 64 single tokens: 3.9 us.  Two vectors per thread were slower (3.1 ->
 // 3.5 us without the launch, 64 tokens).
 #include "attn_ops.cuh"
 
